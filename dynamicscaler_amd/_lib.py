@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 IN_TREE_LIB = os.path.join(HERE, "libdynscaler_hip.so")
 LIB_PATH = os.environ.get("DS_HIP_LIBRARY") or IN_TREE_LIB
 
-DS_F16, DS_F32 = 0, 1
+DS_F16, DS_F32, DS_I8 = 0, 1, 2
 DS_A_DENSE, DS_A_CONV3, DS_A_TCONV = 0, 1, 2
 DS_EPI_GEGLU, DS_EPI_SILU, DS_EPI_OUT_F32, DS_EPI_RES_F32 = 1, 2, 4, 8
 DS_MAX_WINDOWS = 64
@@ -37,6 +37,10 @@ class GemmDesc(C.Structure):
         "t_len", "hw", "ldc", "ldr", "bias_rows", "ldbias", "epilogue", "asym_pad")]
 
 
+class GemmI8Desc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("lda", "ldw", "ldc", "ldr")] + [(n, C.c_int32) for n in ("M", "N", "K", "epilogue")]
+
+
 class UNetConfig(C.Structure):
     """ds_unet_config (include/dynscaler_hip.h)."""
     _fields_ = ([(n, C.c_int32) for n in ("in_channels", "out_channels", "model_channels", "num_res_blocks", "n_channel_mult")]
@@ -46,7 +50,7 @@ class UNetConfig(C.Structure):
                                             "use_image_attention", "fps_cond", "residual_f32", "fold_layernorm", "gn_from_producer", "temporal_selfatt_only")])
 
 
-_vp, _i, _f, _u64, _sz = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_size_t
+_vp, _i, _f, _u64, _sz, _i64 = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_size_t, C.c_int64
 _pp = C.POINTER
 # ds_launch_hook / ds_block_tap (instrumentation of ds_unet_forward)
 LAUNCH_HOOK = C.CFUNCTYPE(None, C.c_void_p, C.c_int, C.c_char_p, C.c_double, C.POINTER(C.c_int32), C.c_int, C.c_void_p)
@@ -107,6 +111,10 @@ SIGNATURES = {
     "ds_clip_preprocess": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "ds_patchify": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "ds_cast_to_f16": (_i, [_vp, _i, _vp, _sz, _vp]),
+    "ds_gemm_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _pp(GemmI8Desc), _vp]),
+    "ds_rmsnorm_rows": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i64, _vp, _i, _i64, _vp, _i, _i, _f, _vp]),
+    "ds_quantize_rows_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i, _i, _vp]),
+    "ds_dequantize_rows_i8": (_i, [_vp, _i64, _vp, _vp, _i, _i64, _i, _i, _vp]),
     "ds_wide_lo_scale": (_f, []),
     "ds_split_f16": (_i, [_vp, _i, _vp, _vp, _sz, _vp]),
     "ds_gemm_wide": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(GemmDesc), _vp]),

@@ -15,14 +15,16 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libdynscaler_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-SOURCES = ["error.cpp", "tile_ops.hip", "gemm.hip", "attention.hip", "norm.hip", "misc.hip", "encoders.hip", "wide.hip", "unet_program.hip"]
+SOURCES = ["error.cpp", "tile_ops.hip", "gemm.hip", "attention.hip", "norm.hip", "misc.hip", "encoders.hip", "wide.hip", "gemm_i8.hip", "rows_i8.hip", "unet_program.hip"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
          "-fno-gpu-rdc", "-ffp-contract=on"]
 
 
 # per-source flags.  attention.hip: -O3's SLP vectoriser pairs adjacent fp32 adds / multiplies into v_pk_*_f32, which cost several
 # times their two halves in the gaps between MFMAs (csrc/attention.hip, DS_ATTN_PK)
-SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"]}
+# gemm_i8.hip, rows_i8.hip: no packed fp32 instructions at all
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"], "gemm_i8.hip": NO_PACKED_F32, "rows_i8.hip": NO_PACKED_F32}
 
 
 def _newer(src_list, target):
@@ -49,7 +51,7 @@ VARIANTS = {"barebarrier": ["-DDS_EXP_BARE_BARRIER"],
             # tuning variants of the 16x16x32 K loop (A/B: tools/gpu_ab.sh): where the LDS-DMA pieces go, how far ahead fragments are read
             # one tile per workgroup, strips over stage 0 (round 3's structure) instead of the persistent big tiles
             "nopersist": ["-DDS_PERSIST=0"],
-            "setprio": ["-DDS_SETPRIO_HI=1"], "nt32": ["-DDS_EXP_NT=11"],
+            "setprio": ["-DDS_SETPRIO_HI=1"], "nt32": ["-DDS_EXP_NT=11"], "nopk": NO_PACKED_F32,
             # fp32 rows: 8 consecutive channels / columns per thread (round 3) instead of two groups of 4 contiguous across the wave
             "now4": ["-DDS_EXP_NO_W4=1"],
             # with ds_gemm_f16_stats (GroupNorm statistics from the producer's epilogue: opt-in feature, profiles/r4_notes.md section 3)

@@ -32,6 +32,7 @@ extern "C" {
 
 #define DS_F16 0
 #define DS_F32 1
+#define DS_I8 2    /* 8-bit integers with an fp32 scale per row (the W8A8 operators only) */
 
 const char* ds_last_error(void);
 /* ABI version of this header; bumped on any signature or struct-layout change (round 4: 2 -- ds_unet_config gained
@@ -338,6 +339,37 @@ int ds_rows_to_ncthw(const void* y, int y_dtype, int ldy, void* out, int out_dty
 int ds_timestep_embedding(const int64_t* t, void* out, int n, int dim, void* stream);
 /* y = silu(x), fp16 elementwise (emb_layers SiLU, openaimodel3d.py:172-178). */
 int ds_silu_f16(const void* x, void* y, size_t n, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * W8A8: 8-bit integer operands with one fp32 scale per row -- of the activations a token's, of the weights an output channel's.  A
+ * transformer block's chain: ds_rmsnorm_rows (8-bit) -> ds_gemm_i8 (GEGLU) -> ds_quantize_rows_i8 -> ds_gemm_i8 (+ residual).
+ * Row strides (ld*) are in elements, >= the row's length, otherwise free; pointers have to be aligned to their element only.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct ds_gemm_i8_desc {
+    int64_t lda, ldw, ldc, ldr;   /* row strides of A, W, out and residual in elements                          */
+    int32_t M, N, K;              /* any sizes, 0 included; K <= 131071 (the sums are exact 32-bit integers)    */
+    int32_t epilogue;             /* DS_EPI_* flags: GEGLU (N % 64 == 0, no residual, W rows and bias in
+                                     ds_gemm_f16's 32-row groups, out has N / 2 columns), SILU, OUT_F32, RES_F32 */
+} ds_gemm_i8_desc;
+/* out[m][n] = act(a_scale[m] * w_scale[n] * sum_k A[m][k] W[n][k] + bias[n]) + residual[m][n]
+ * A int8 [M][lda], W int8 [N][ldw], a_scale [M], w_scale [N], bias [N] or NULL (fp32); residual fp16 (fp32 with DS_EPI_RES_F32) or NULL;
+ * out fp16 (fp32 with DS_EPI_OUT_F32).  The sum is exact: results do not depend on the tile shape or on the rows of the launch.  residual
+ * may be out itself (the same pointer, type and stride).  The products it stands next to: ds_gemm_f16's dense ones (nn.Linear,
+ * attention.py:54-57, 379, 399). */
+int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale, const float* w_scale, const float* bias, const void* residual,
+               void* out, const ds_gemm_i8_desc* desc, void* stream);
+/* h = x + residual; t = h * gamma; root = 1 / sqrt(mean(h^2) + eps) over each row of C values; y = t * root as fp16 / fp32, or (y_dtype
+ * DS_I8) q = rint(127 t / max|t|) with scale[row] = max|t| * root / 127.  q is the correctly rounded quotient (halves to even, formed in
+ * 64 bits).  residual may be NULL (no addition); sum (NULL: not wanted) receives h in the residual's type, the norm reads the unrounded
+ * h.  8-bit rows: all t zero -> q = 0, scale = 0; a NaN or an infinity in the row -> q = 0, scale = NaN.  eps > 0.
+ * In place: sum may be residual, and a fp16 / fp32 y may be x (same type and stride). */
+int ds_rmsnorm_rows(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr, const float* gamma,
+                    void* sum, int64_t lds, void* y, int y_dtype, int64_t ldy, float* scale, int rows, int C, float eps, void* stream);
+/* q = rint(127 x / max|x|), scale[row] = max|x| / 127 over each row of C values (activations without a norm in front; weights, row =
+ * output channel).  Rounding, zeros and non-finite rows as in ds_rmsnorm_rows. */
+int ds_quantize_rows_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int rows, int C, void* stream);
+/* y = q * scale[row], rounded once to fp16 / fp32. */
+int ds_dequantize_rows_i8(const int8_t* q, int64_t ldq, const float* scale, void* y, int y_dtype, int64_t ldy, int rows, int C, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * The WIDE operand mode (round 5): the same UNet blocks evaluated as an fp32 computation -- every activation stored in fp32, every

@@ -1,0 +1,150 @@
+"""The W8A8 operators' refusals: no call below reaches a device."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+from dynamicscaler_amd import _lib, ops
+from dynamicscaler_amd._lib import DS_EPI_GEGLU, DS_EPI_SILU, DsError
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+F16, F32, I8 = torch.float16, torch.float32, torch.int8
+
+
+def product(**kw):
+    c = dict(A=torch.zeros((4, 32), dtype=I8), W=torch.zeros((64, 32), dtype=I8), a_scale=torch.ones(4), w_scale=torch.ones(64))
+    c.update(kw)
+    return c
+
+
+@pytest.mark.parametrize("change,says", [
+    (dict(A=torch.zeros((4, 32))), "gemm_i8\\(A\\).*float32"),
+    (dict(A=torch.zeros((4, 32, 1), dtype=I8)), "\\[rows, columns\\]"),
+    (dict(W=torch.zeros((64, 31), dtype=I8)), "gemm_i8\\(W\\).*expected 64 x 32"),
+    (dict(A=torch.zeros((32, 4), dtype=I8).t()), "contiguous"),
+    (dict(A=torch.zeros((1, 32), dtype=I8).expand(4, 32)), "overlap"),
+    (dict(a_scale=torch.ones(5)), "a_scale.*4 values"),
+    (dict(a_scale=torch.ones(4, dtype=F16)), "a_scale"),
+    (dict(a_scale=torch.ones(8)[::2]), "a_scale"),
+    (dict(w_scale=torch.ones(1)), "w_scale.*64 values"),
+    (dict(w_scale=torch.ones((64, 1))), "w_scale"),
+    (dict(bias=torch.ones(63)), "bias"),
+    (dict(residual=torch.zeros((4, 63), dtype=F16)), "residual.*expected 4 x 64"),
+    (dict(residual=torch.zeros((4, 64), dtype=torch.float64)), "residual"),
+    (dict(out=torch.zeros((4, 64), dtype=I8)), "out"),
+    (dict(out=torch.zeros((1, 64), dtype=F16).expand(4, 64)), "overlap"),
+    (dict(out=torch.zeros((4, 64), dtype=F16), epilogue=DS_EPI_GEGLU), "out.*expected 4 x 32"),
+    (dict(out_dtype=torch.bfloat16), "out_dtype"),
+    (dict(), "no CPU fallback"),
+])
+def test_product_refuses(change, says):
+    with pytest.raises(DsError, match=says):
+        ops.gemm_i8(**product(**change))
+
+
+X = torch.zeros((4, 32), dtype=F16)
+
+
+@pytest.mark.parametrize("call,says", [
+    (lambda: ops.rmsnorm(X.to(torch.bfloat16), torch.ones(32)), "x"),
+    (lambda: ops.rmsnorm(X, torch.ones(31)), "gamma.*32 values"),
+    (lambda: ops.rmsnorm(X, torch.ones(32, dtype=F16)), "gamma"),
+    (lambda: ops.rmsnorm(X, torch.ones(32), residual=torch.zeros((3, 32))), "residual.*expected 4 x 32"),
+    (lambda: ops.rmsnorm(X, torch.ones(32), residual=X, sum_out=torch.zeros((4, 32))), "sum_out.*float32"),
+    (lambda: ops.rmsnorm(X, torch.ones(32), sum_out=X), "without a residual"),
+    (lambda: ops.rmsnorm(X, torch.ones(32), out=torch.zeros((4, 32), dtype=I8)), "out"),
+    (lambda: ops.rmsnorm(X, torch.ones(32), out_dtype=I8), "out_dtype"),
+    (lambda: ops.rmsnorm(X[:, :0], torch.ones(0)), "without values"),
+    (lambda: ops.rmsnorm_i8(X, torch.ones(32), out=X), "out"),
+    (lambda: ops.rmsnorm_i8(X, torch.ones(32), scale=torch.ones(3)), "scale.*4 values"),
+    (lambda: ops.rmsnorm_i8(X, torch.ones(32)), "no CPU fallback"),
+    (lambda: ops.quantize_rows_i8(X.to(I8)), "x"),
+    (lambda: ops.quantize_rows_i8(X[:, :0]), "without values"),
+    (lambda: ops.quantize_rows_i8(X, out=torch.zeros((4, 33), dtype=I8)), "expected 4 x 32"),
+    (lambda: ops.quantize_rows_i8(X, scale=torch.ones((4, 1))), "scale"),
+    (lambda: ops.quantize_rows_i8(X.t()[:, :2]), "contiguous"),
+    (lambda: ops.quantize_rows_i8(X), "no CPU fallback"),
+    (lambda: ops.dequantize_rows_i8(X, torch.ones(4)), "q"),
+    (lambda: ops.dequantize_rows_i8(X.to(I8), torch.ones(5)), "scale"),
+    (lambda: ops.dequantize_rows_i8(X.to(I8), torch.ones(4), dtype=I8), "dtype"),
+    (lambda: ops.dequantize_rows_i8(X.to(I8), torch.ones(4), out=X[:3]), "expected 4 x 32"),
+    (lambda: ops.dequantize_rows_i8(X.to(I8), torch.ones(4)), "no CPU fallback"),
+])
+def test_rows_refuse(call, says):
+    with pytest.raises(DsError, match=says):
+        call()
+
+
+def refused(rc, says):
+    assert rc == -1 and re.search(says, _lib.load().ds_last_error().decode()), _lib.load().ds_last_error()
+
+
+P = 1 << 20      # stands for an aligned device address; a refused call does not follow it
+
+
+@pytest.mark.parametrize("fields,args,says", [
+    (dict(K=131072, lda=131072, ldw=131072), {}, "131071"),
+    (dict(M=-1), {}, "negative"),
+    (dict(epilogue=16), {}, "epilogue"),
+    (dict(epilogue=DS_EPI_GEGLU | DS_EPI_SILU), {}, "exclude"),
+    (dict(epilogue=DS_EPI_GEGLU, N=96, ldc=96), {}, "N % 64"),
+    (dict(epilogue=DS_EPI_GEGLU, ldr=64), dict(residual=P), "no residual"),
+    (dict(lda=31), {}, "row stride"),
+    (dict(ldw=0), {}, "row stride"),
+    (dict(ldc=63), {}, "row stride"),
+    (dict(ldr=63), dict(residual=P), "row stride"),
+    ({}, dict(A=0), "NULL"),
+    ({}, dict(w_scale=0), "NULL"),
+    ({}, dict(out=0), "NULL"),
+    ({}, dict(out=P + 1), "aligned"),
+    (dict(ldr=64, epilogue=8), dict(residual=P + 2), "aligned"),
+    ({}, dict(bias=P + 2), "aligned"),
+])
+def test_product_c_entry_refuses(fields, args, says):
+    d = _lib.GemmI8Desc()
+    for k, v in dict(dict(M=4, N=64, K=32, lda=32, ldw=32, ldc=64, ldr=0, epilogue=0), **fields).items():
+        setattr(d, k, v)
+    a = dict(dict(A=P, W=P, a_scale=P, w_scale=P, bias=0, residual=0, out=P), **args)
+    refused(_lib.load().ds_gemm_i8(a["A"], a["W"], a["a_scale"], a["w_scale"], a["bias"], a["residual"], a["out"], C.byref(d), 0), says)
+
+
+def test_product_c_entry_refuses_no_desc_and_accepts_nothing_to_do():
+    lib = _lib.load()
+    refused(lib.ds_gemm_i8(P, P, P, P, 0, 0, P, None, 0), "desc")
+    d = _lib.GemmI8Desc(M=0, N=64, K=32, lda=32, ldw=32, ldc=64)
+    assert lib.ds_gemm_i8(P, P, P, P, 0, 0, P, C.byref(d), 0) == 0
+
+
+NORM = dict(x=P, xt=0, ldx=32, r=P, rt=0, ldr=32, g=P, s=P, lds=32, y=P, yt=2, ldy=32, scale=P, rows=4, C=32, eps=1e-6)
+
+
+@pytest.mark.parametrize("change,says", [
+    (dict(C=0), "C 0"), (dict(rows=-1), "rows -1"), (dict(xt=2), "type 2"), (dict(rt=3), "type"), (dict(yt=5), "result type"),
+    (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"), (dict(x=0), "NULL"), (dict(g=0), "NULL"),
+    (dict(scale=0), "NULL"), (dict(r=0), "without a residual"), (dict(ldx=31), "row stride"), (dict(lds=31), "row stride"),
+    (dict(ldr=0), "row stride"), (dict(ldy=31), "row stride"), (dict(x=P + 1), "aligned"), (dict(r=P + 2, rt=1), "aligned"), (dict(g=P + 2), "aligned")])
+def test_norm_c_entry_refuses(change, says):
+    c = dict(NORM, **change)
+    refused(_lib.load().ds_rmsnorm_rows(c["x"], c["xt"], c["ldx"], c["r"], c["rt"], c["ldr"], c["g"], c["s"], c["lds"], c["y"], c["yt"], c["ldy"],
+                                        c["scale"], c["rows"], c["C"], c["eps"], 0), says)
+
+
+@pytest.mark.parametrize("args,says", [((P, 2, 32, P, 32, P, 4, 32), "type"), ((P, 0, 31, P, 32, P, 4, 32), "row stride"), ((P, 0, 32, 0, 32, P, 4, 32), "NULL"),
+                                       ((P, 0, 32, P, 32, P + 2, 4, 32), "aligned"), ((P, 0, 32, P, 32, P, 4, 0), "C 0")])
+def test_quantize_c_entry_refuses(args, says):
+    refused(_lib.load().ds_quantize_rows_i8(*args, 0), says)
+
+
+@pytest.mark.parametrize("args,says", [((P, 32, P, P, 2, 32, 4, 32), "type"), ((P, 31, P, P, 0, 32, 4, 32), "row stride"), ((P, 32, 0, P, 0, 32, 4, 32), "NULL"),
+                                       ((P, 32, P, P + 2, 1, 32, 4, 32), "aligned")])
+def test_dequantize_c_entry_refuses(args, says):
+    refused(_lib.load().ds_dequantize_rows_i8(*args, 0), says)
+
+
+def test_desc_layout_matches_the_header():
+    header = re.sub(r"/\*.*?\*/", "", open(os.path.join(REPO, "include", "dynscaler_hip.h")).read(), flags=re.S)
+    body = re.search(r"typedef struct ds_gemm_i8_desc \{(.*?)\} ds_gemm_i8_desc;", header, flags=re.S).group(1)
+    fields = [(n.strip(), t) for t, names in re.findall(r"(int(?:32|64)_t) ([^;]+);", body) for n in names.split(",")]
+    assert [(n, {C.c_int64: "int64_t", C.c_int32: "int32_t"}[t]) for n, t in _lib.GemmI8Desc._fields_] == fields
