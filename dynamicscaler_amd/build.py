@@ -51,7 +51,9 @@ VARIANTS = {"barebarrier": ["-DDS_EXP_BARE_BARRIER"],
             # tuning variants of the 16x16x32 K loop (A/B: tools/gpu_ab.sh): where the LDS-DMA pieces go, how far ahead fragments are read
             # one tile per workgroup, strips over stage 0 (round 3's structure) instead of the persistent big tiles
             "nopersist": ["-DDS_PERSIST=0"],
-            "setprio": ["-DDS_SETPRIO_HI=1"], "nt32": ["-DDS_EXP_NT=11"], "nopk": NO_PACKED_F32,
+            "setprio": ["-DDS_SETPRIO_HI=1"], "nt32": ["-DDS_EXP_NT=11"],
+            # every source without packed fp32 (the older ones too): +1.0 % per cfg3 step, other last bits (fused multiply-adds pair differently)
+            "nopk": NO_PACKED_F32,
             # fp32 rows: 8 consecutive channels / columns per thread (round 3) instead of two groups of 4 contiguous across the wave
             "now4": ["-DDS_EXP_NO_W4=1"],
             # with ds_gemm_f16_stats (GroupNorm statistics from the producer's epilogue: opt-in feature, profiles/r4_notes.md section 3)

@@ -47,11 +47,181 @@ __device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
     return v;
 }
 
-// One workgroup per row, the row read once for the sums and once for the result.
+// 8 values of a row as they lie in memory (any address that is a multiple of the element's size), as fp32 (exact for fp16), and back
+typedef f16x8 __attribute__((aligned(2))) f16x8_u;
+typedef f32x4 __attribute__((aligned(4))) f32x4_u;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 __attribute__((aligned(1))) u32x2_u;
+
+template <typename T> struct Chunk;
+template <> struct Chunk<f16> {
+    f16x8 v;
+    __device__ __forceinline__ void zero() { v = f16x8{0, 0, 0, 0, 0, 0, 0, 0}; }
+    __device__ __forceinline__ void load(const f16* p) { v = *reinterpret_cast<const f16x8_u*>(p); }
+    __device__ __forceinline__ void hold() { asm volatile("" : "+v"(v)); }
+    __device__ __forceinline__ float at(int j) const { return (float)v[j]; }
+    __device__ __forceinline__ void set(int j, double x) { v[j] = (f16)(float)x; }
+    __device__ __forceinline__ void store(f16* p) const { *reinterpret_cast<f16x8_u*>(p) = v; }
+};
+template <> struct Chunk<float> {
+    f32x4 v[2];
+    __device__ __forceinline__ void zero() { v[0] = v[1] = f32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void hold() { asm volatile("" : "+v"(v[0]), "+v"(v[1])); }
+    __device__ __forceinline__ void load(const float* p) {
+        v[0] = *reinterpret_cast<const f32x4_u*>(p);
+        v[1] = *reinterpret_cast<const f32x4_u*>(p + 4);
+    }
+    __device__ __forceinline__ float at(int j) const { return v[j >> 2][j & 3]; }
+    __device__ __forceinline__ void set(int j, double x) { v[j >> 2][j & 3] = (float)x; }
+    __device__ __forceinline__ void store(float* p) const {
+        *reinterpret_cast<f32x4_u*>(p) = v[0];
+        *reinterpret_cast<f32x4_u*>(p + 4) = v[1];
+    }
+};
+template <> struct Chunk<int8_t> {
+    u32x2 v;
+    __device__ __forceinline__ void zero() { v = u32x2{0, 0}; }
+    __device__ __forceinline__ void put(int j, int q) { v[j >> 2] |= (unsigned)(q & 255) << (8 * (j & 3)); }
+    __device__ __forceinline__ void store(int8_t* p) const { *reinterpret_cast<u32x2_u*>(p) = v; }
+};
+
+// Rows of 8 ... 8 T V values: a team of T lanes (of one wave for T <= 64, a whole workgroup above) keeps a row in registers -- read once,
+// reduced twice, written once; lane i of the team holds chunks i, i + T, ... of 8 values, so a load covers 16 T contiguous bytes (fp16).
+// A row's last chunk always ends at the row's end: where C % 8 != 0 it overlaps the one before, counts its own values only in the sum, and
+// stores the same bits over the shared ones (every load of a row comes before its first store, also where sum / y lie over an input).
+// A team walks rows `grid` apart and keeps its part of gamma.
+template <typename X, typename R, typename Y, bool NORM, bool RES, int T, int V>
+__global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
+    constexpr int TEAMS = 256 / T, WAVES = T / 64;
+    constexpr bool I8 = sizeof(Y) == 1;
+    __shared__ double s_sum[2][WAVES > 1 ? WAVES : 1], s_top[2][WAVES > 1 ? WAVES : 1];
+    const int tid = threadIdx.x, lane = tid % T, team = tid / T;
+    const int C = p.C;
+    auto chunk = [&](int v) { return (v * T + lane) * 8; };            // where the lane's chunk v would begin: it has one if that is < C,
+    auto at = [&](int v) { return min(chunk(v), C - 8); };              // and it begins here
+    Chunk<float> g[V];
+    bool bad_g = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if constexpr (NORM) {
+            g[v].zero();
+            if (chunk(v) < C) g[v].load(p.g + at(v));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) bad_g |= !(fabsf(g[v].at(j)) < __builtin_huge_valf());
+        }
+    }
+    int turn = 0;
+    for (long row0 = (long)blockIdx.x * TEAMS; row0 < rows; row0 += (long)gridDim.x * TEAMS, turn ^= 1) {
+        const long row = row0 + team;
+        const bool live = row < rows;          // teams of one wave: the reductions below need every lane
+        const long rr = live ? row : rows - 1;
+        const X* x = reinterpret_cast<const X*>(p.x) + rr * p.ldx;
+        const R* r = reinterpret_cast<const R*>(p.r) + rr * p.ldr;
+        Chunk<X> cx[V];
+        Chunk<R> cr[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (v * T * 8 >= C) break;
+            cx[v].zero();
+            if constexpr (RES) cr[v].zero();
+            if (chunk(v) < C) {
+                cx[v].load(x + at(v));
+                if constexpr (RES) cr[v].load(r + at(v));
+            }
+        }
+        auto h_of = [&](int v, int j) {
+            double h = (double)cx[v].at(j);
+            if constexpr (RES) h += (double)cr[v].at(j);
+            return h;
+        };
+        auto t_of = [&](int v, int j) { return NORM ? h_of(v, j) * (double)g[v].at(j) : h_of(v, j); };
+        if constexpr (NORM) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) g[v].hold();      // gamma stays in 32 bits between the rows
+        }
+        double sum = 0.0, top = 0.0;
+        bool bad = bad_g;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (v * T * 8 >= C) break;
+            if constexpr (NORM) {
+                const int shared = chunk(v) < C ? chunk(v) - at(v) : 0;       // values that belong to the chunk before
+                if (shared == 0) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { const double h = h_of(v, j); sum = fma(h, h, sum); }
+                } else {
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) { const double h = j < shared ? 0.0 : h_of(v, j); sum = fma(h, h, sum); }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (NORM) {
+                    if constexpr (I8) top = fmax(top, fabs(t_of(v, j)));
+                } else {
+                    const float a = fabsf(cx[v].at(j));
+                    bad |= !(a < __builtin_huge_valf());
+                    top = fmax(top, (double)a);
+                }
+            }
+        }
+        if (I8 && bad) top = __builtin_nan("");
+#pragma unroll
+        for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) {
+            if constexpr (NORM) sum += __shfl_xor(sum, o);
+            if constexpr (I8) {
+                const double u = __shfl_xor(top, o);
+                top = top < u || u != u ? u : top;           // NaN stays
+            }
+        }
+        if constexpr (T > 64) {
+            if ((tid & 63) == 0) { s_sum[turn][tid >> 6] = sum; s_top[turn][tid >> 6] = top; }
+            __syncthreads();                    // two copies in turn: the next row's stores come a barrier after this row's loads
+            sum = s_sum[turn][0];
+            top = s_top[turn][0];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) {
+                sum += s_sum[turn][w];
+                const double u = s_top[turn][w];
+                top = top < u || u != u ? u : top;
+            }
+        }
+        const double root = NORM ? 1.0 / sqrt(sum / C + (double)p.eps) : 1.0;
+        const bool off = I8 && (!(sum < __builtin_huge_val()) || !(top < __builtin_huge_val()));
+        const double inv = I8 && top > 0.0 && !off ? 127.0 / top : 0.0;
+        if (I8 && live && lane == 0) p.scale[row] = off ? __builtin_nanf("") : (float)(top * root / 127.0);
+        Y* y = reinterpret_cast<Y*>(p.y) + rr * p.ldy;
+        R* hs = reinterpret_cast<R*>(p.h) + rr * p.ldh;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (v * T * 8 >= C) break;
+            cx[v].hold();                    // the raw values stay in registers, their 64-bit forms are made again (half the registers)
+            if constexpr (RES) cr[v].hold();
+            if constexpr (NORM) g[v].hold();
+            const bool mine = live && chunk(v) < C;
+            Chunk<Y> cy;
+            cy.zero();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (I8) cy.put(j, inv > 0.0 ? quantum(t_of(v, j), top, inv) : 0);
+                else cy.set(j, t_of(v, j) * root);
+            }
+            if (mine) cy.store(y + at(v));
+            if constexpr (RES) {
+                Chunk<R> ch;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ch.set(j, h_of(v, j));
+                if (mine && p.h) ch.store(hs + at(v));
+            }
+        }
+    }
+}
+
+// Longer rows, and rows of less than 8 values: one workgroup per row, the row read for the sums and again for the result.
 template <typename X, typename R, typename Y, bool NORM>
-__global__ void __launch_bounds__(256) rows_kernel(RowsArgs p) {
-    __shared__ double s_sum[4];
-    __shared__ unsigned long long s_top[4];
+__global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p) {
+    __shared__ double s_sum[16];
+    __shared__ unsigned long long s_top[16];
     const long row = blockIdx.x;
     const int tid = threadIdx.x;
     const X* x = reinterpret_cast<const X*>(p.x) + row * p.ldx;
@@ -59,7 +229,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs p) {
     auto h_of = [&](int c) { return r ? as_f64(x[c]) + as_f64(r[c]) : as_f64(x[c]); };
     double sum = 0.0;
     unsigned long long top = 0;       // bit patterns of non-negative doubles order like the values, infinities and NaN above them
-    for (int c = tid; c < p.C; c += 256) {
+    for (int c = tid; c < p.C; c += blockDim.x) {
         const double h = h_of(c);
         sum += h * h;
         const double t = NORM ? h * (double)p.g[c] : h;
@@ -70,9 +240,11 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs p) {
     top = wave_max(top);
     if ((tid & 63) == 0) { s_sum[tid >> 6] = sum; s_top[tid >> 6] = top; }
     __syncthreads();
-    sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-    top = s_top[0];
-    for (int w = 1; w < 4; ++w) top = s_top[w] > top ? s_top[w] : top;
+    sum = 0.0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+        sum += s_sum[w];
+        top = s_top[w] > top ? s_top[w] : top;
+    }
     const double root = NORM ? 1.0 / sqrt(sum / p.C + (double)p.eps) : 1.0;
     const double dtop = __longlong_as_double(top);
     if constexpr (sizeof(Y) == 1) {
@@ -80,7 +252,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs p) {
         const double inv = dtop > 0.0 && !bad ? 127.0 / dtop : 0.0;
         int8_t* q = reinterpret_cast<int8_t*>(p.y) + row * p.ldy;
         if (tid == 0) p.scale[row] = bad ? __builtin_nanf("") : (float)(dtop * root / 127.0);
-        for (int c = tid; c < p.C; c += 256) {
+        for (int c = tid; c < p.C; c += blockDim.x) {
             const double h = h_of(c);
             q[c] = (int8_t)(inv > 0.0 ? quantum(NORM ? h * (double)p.g[c] : h, dtop, inv) : 0);
             if constexpr (NORM) {
@@ -89,7 +261,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs p) {
         }
     } else {
         Y* y = reinterpret_cast<Y*>(p.y) + row * p.ldy;
-        for (int c = tid; c < p.C; c += 256) {
+        for (int c = tid; c < p.C; c += blockDim.x) {
             const double h = h_of(c);
             y[c] = (Y)(float)(h * root * (double)p.g[c]);
             if (p.h) reinterpret_cast<R*>(p.h)[row * p.ldh + c] = (R)h;
@@ -97,23 +269,50 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs p) {
     }
 }
 
+// Teams of 1 << shift lanes per row, 8 values per lane and turn.
 template <typename Y>
-__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, long ldq, const float* scale, Y* y, long ldy, int C) {
-    const long row = blockIdx.x;
+__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C, int shift) {
+    const long row = (long)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & ((1 << shift) - 1);
     const float s = scale[row];
-    for (int c = threadIdx.x; c < C; c += 256) y[row * ldy + c] = (Y)((float)q[row * ldq + c] * s);
+    const int8_t* src = q + row * ldq;
+    Y* dst = y + row * ldy;
+    for (int c = lane * 8; c < C; c += 8 << shift) {
+        if (c + 8 <= C) {
+            const u32x2 v = *reinterpret_cast<const u32x2_u*>(src + c);
+            Chunk<Y> cy;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) cy.set(j, (float)((int)(v[j >> 2] << (24 - 8 * (j & 3))) >> 24) * s);
+            cy.store(dst + c);
+        } else {
+            for (int j = c; j < C; ++j) dst[j] = (Y)((float)src[j] * s);
+        }
+    }
 }
 
 bool rows_dtype(int t) { return t == DS_F16 || t == DS_F32; }
 bool aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == DS_I8 ? 0 : dtype == DS_F32 ? 3 : 1)) == 0; }
 
-template <typename X, typename R, bool NORM>
-void launch_y(const RowsArgs& p, int y_dtype, int rows, hipStream_t st) {
-    if (y_dtype == DS_I8) rows_kernel<X, R, int8_t, NORM><<<rows, 256, 0, st>>>(p);
-    else if constexpr (NORM) {
-        if (y_dtype == DS_F16) rows_kernel<X, R, f16, NORM><<<rows, 256, 0, st>>>(p);
-        else rows_kernel<X, R, float, NORM><<<rows, 256, 0, st>>>(p);
-    }
+template <typename X, typename R, typename Y, bool NORM, bool RES>
+void launch_rows(const RowsArgs& p, int rows, hipStream_t st) {
+    // the smallest team whose four chunks a lane hold the row; teams walk several rows once the chip is full (16 waves a CU)
+    constexpr int V = 4, FULL = 256 * 4;
+    auto grid = [&](int teams) { const int n = ds_cdiv(rows, teams); return n < FULL ? n : FULL; };
+    if (p.C < 8) rows_long_kernel<X, R, Y, NORM><<<rows, 64, 0, st>>>(p);
+    else if (p.C <= 8 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 8, V><<<grid(32), 256, 0, st>>>(p, rows);
+    else if (p.C <= 16 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 16, V><<<grid(16), 256, 0, st>>>(p, rows);
+    else if (p.C <= 32 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 32, V><<<grid(8), 256, 0, st>>>(p, rows);
+    else if (p.C <= 64 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 64, V><<<grid(4), 256, 0, st>>>(p, rows);
+    else if (p.C <= 256 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 256, V><<<grid(1), 256, 0, st>>>(p, rows);
+    else rows_long_kernel<X, R, Y, NORM><<<rows, 1024, 0, st>>>(p);
+}
+
+template <typename X, typename R, bool RES>
+void launch_norm(const RowsArgs& p, int y_dtype, int rows, hipStream_t st) {
+    if (y_dtype == DS_I8) launch_rows<X, R, int8_t, true, RES>(p, rows, st);
+    else if (y_dtype == DS_F16) launch_rows<X, R, f16, true, RES>(p, rows, st);
+    else launch_rows<X, R, float, true, RES>(p, rows, st);
 }
 
 }  // namespace
@@ -132,11 +331,17 @@ extern "C" int ds_rmsnorm_rows(const void* x, int x_dtype, int64_t ldx, const vo
                  "ds_rmsnorm_rows: a pointer is not aligned to its element");
     const RowsArgs p{x, residual, gamma, sum, y, scale, ldx, ldr, lds, ldy, C, eps};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const bool xf = x_dtype == DS_F32, rf = residual && r_dtype == DS_F32;
-    if (xf && rf) launch_y<float, float, true>(p, y_dtype, rows, st);
-    else if (xf) launch_y<float, f16, true>(p, y_dtype, rows, st);
-    else if (rf) launch_y<f16, float, true>(p, y_dtype, rows, st);
-    else launch_y<f16, f16, true>(p, y_dtype, rows, st);
+    const bool xf = x_dtype == DS_F32, rf = r_dtype == DS_F32;
+    if (!residual) {
+        if (xf) launch_norm<float, f16, false>(p, y_dtype, rows, st);
+        else launch_norm<f16, f16, false>(p, y_dtype, rows, st);
+    } else if (rf) {
+        if (xf) launch_norm<float, float, true>(p, y_dtype, rows, st);
+        else launch_norm<f16, float, true>(p, y_dtype, rows, st);
+    } else {
+        if (xf) launch_norm<float, f16, true>(p, y_dtype, rows, st);
+        else launch_norm<f16, f16, true>(p, y_dtype, rows, st);
+    }
     DS_CHECK_LAUNCH("ds_rmsnorm_rows");
     return DS_OK;
 }
@@ -150,8 +355,8 @@ extern "C" int ds_quantize_rows_i8(const void* x, int x_dtype, int64_t ldx, int8
     DS_CHECK_ARG(aligned(x, x_dtype) && aligned(scale, DS_F32), "ds_quantize_rows_i8: a pointer is not aligned to its element");
     const RowsArgs p{x, nullptr, nullptr, nullptr, q, scale, ldx, 0, 0, ldq, C, 0.0f};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (x_dtype == DS_F32) launch_y<float, float, false>(p, DS_I8, rows, st);
-    else launch_y<f16, f16, false>(p, DS_I8, rows, st);
+    if (x_dtype == DS_F32) launch_rows<float, f16, int8_t, false, false>(p, rows, st);
+    else launch_rows<f16, f16, int8_t, false, false>(p, rows, st);
     DS_CHECK_LAUNCH("ds_quantize_rows_i8");
     return DS_OK;
 }
@@ -164,8 +369,11 @@ extern "C" int ds_dequantize_rows_i8(const int8_t* q, int64_t ldq, const float* 
     DS_CHECK_ARG(ldq >= C && ldy >= C, "ds_dequantize_rows_i8: a row stride is shorter than C %d", C);
     DS_CHECK_ARG(aligned(y, y_dtype) && aligned(scale, DS_F32), "ds_dequantize_rows_i8: a pointer is not aligned to its element");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (y_dtype == DS_F32) dequant_kernel<float><<<rows, 256, 0, st>>>(q, ldq, scale, (float*)y, ldy, C);
-    else dequant_kernel<f16><<<rows, 256, 0, st>>>(q, ldq, scale, (f16*)y, ldy, C);
+    int shift = 3;                 // the smallest team that holds the row in one turn, at most a workgroup
+    while (shift < 8 && (8 << shift) < C) ++shift;
+    const int grid = ds_cdiv(rows, 256 >> shift);
+    if (y_dtype == DS_F32) dequant_kernel<float><<<grid, 256, 0, st>>>(q, ldq, scale, (float*)y, ldy, rows, C, shift);
+    else dequant_kernel<f16><<<grid, 256, 0, st>>>(q, ldq, scale, (f16*)y, ldy, rows, C, shift);
     DS_CHECK_LAUNCH("ds_dequantize_rows_i8");
     return DS_OK;
 }
