@@ -317,8 +317,11 @@ void launch_norm(const RowsArgs& p, int y_dtype, int rows, hipStream_t st) {
 
 }  // namespace
 
-extern "C" int ds_rmsnorm_rows(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr, const float* gamma,
-                               void* sum, int64_t lds, void* y, int y_dtype, int64_t ldy, float* scale, int rows, int C, float eps, void* stream) {
+extern "C" int ds_rmsnorm_rows(const void* x, const void* residual, const float* gamma, void* sum, void* y, float* scale, const ds_rmsnorm_desc* desc, void* stream) {
+    DS_CHECK_ARG(desc, "ds_rmsnorm_rows: desc is NULL");
+    const int64_t ldx = desc->ldx, ldr = desc->ldr, lds = desc->lds, ldy = desc->ldy;
+    const int rows = desc->rows, C = desc->C, x_dtype = desc->x_dtype, r_dtype = desc->r_dtype, y_dtype = desc->y_dtype;
+    const float eps = desc->eps;
     DS_CHECK_ARG(rows >= 0 && C >= 1, "ds_rmsnorm_rows: rows %d, C %d", rows, C);
     DS_CHECK_ARG(rows_dtype(x_dtype) && (!residual || rows_dtype(r_dtype)), "ds_rmsnorm_rows: x / residual type %d / %d", x_dtype, r_dtype);
     DS_CHECK_ARG(y_dtype == DS_I8 || rows_dtype(y_dtype), "ds_rmsnorm_rows: result type %d", y_dtype);

@@ -363,8 +363,14 @@ int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale, const flo
  * 64 bits).  residual may be NULL (no addition); sum (NULL: not wanted) receives h in the residual's type, the norm reads the unrounded
  * h.  8-bit rows: all t zero -> q = 0, scale = 0; a NaN or an infinity in the row -> q = 0, scale = NaN.  eps > 0.
  * In place: sum may be residual, and a fp16 / fp32 y may be x (same type and stride). */
-int ds_rmsnorm_rows(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr, const float* gamma,
-                    void* sum, int64_t lds, void* y, int y_dtype, int64_t ldy, float* scale, int rows, int C, float eps, void* stream);
+typedef struct ds_rmsnorm_desc {
+    int64_t ldx, ldr, lds, ldy;               /* row strides of x, residual, sum and y in elements              */
+    int32_t rows, C;
+    int32_t x_dtype, r_dtype, y_dtype;        /* DS_F16 / DS_F32; y also DS_I8; sum has the residual's type     */
+    float eps;
+} ds_rmsnorm_desc;
+int ds_rmsnorm_rows(const void* x, const void* residual, const float* gamma, void* sum, void* y, float* scale, const ds_rmsnorm_desc* desc,
+                    void* stream);
 /* q = rint(127 x / max|x|), scale[row] = max|x| / 127 over each row of C values (activations without a norm in front; weights, row =
  * output channel).  Rounding, zeros and non-finite rows as in ds_rmsnorm_rows. */
 int ds_quantize_rows_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int rows, int C, void* stream);

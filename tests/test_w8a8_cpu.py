@@ -127,8 +127,12 @@ NORM = dict(x=P, xt=0, ldx=32, r=P, rt=0, ldr=32, g=P, s=P, lds=32, y=P, yt=2, l
     (dict(ldr=0), "row stride"), (dict(ldy=31), "row stride"), (dict(x=P + 1), "aligned"), (dict(r=P + 2, rt=1), "aligned"), (dict(g=P + 2), "aligned")])
 def test_norm_c_entry_refuses(change, says):
     c = dict(NORM, **change)
-    refused(_lib.load().ds_rmsnorm_rows(c["x"], c["xt"], c["ldx"], c["r"], c["rt"], c["ldr"], c["g"], c["s"], c["lds"], c["y"], c["yt"], c["ldy"],
-                                        c["scale"], c["rows"], c["C"], c["eps"], 0), says)
+    d = _lib.RmsnormDesc(c["ldx"], c["ldr"], c["lds"], c["ldy"], c["rows"], c["C"], c["xt"], c["rt"], c["yt"], c["eps"])
+    refused(_lib.load().ds_rmsnorm_rows(c["x"], c["r"], c["g"], c["s"], c["y"], c["scale"], C.byref(d), 0), says)
+
+
+def test_norm_c_entry_refuses_no_desc():
+    refused(_lib.load().ds_rmsnorm_rows(P, 0, P, 0, P, P, None, 0), "desc")
 
 
 @pytest.mark.parametrize("args,says", [((P, 2, 32, P, 32, P, 4, 32), "type"), ((P, 0, 31, P, 32, P, 4, 32), "row stride"), ((P, 0, 32, 0, 32, P, 4, 32), "NULL"),
@@ -143,8 +147,11 @@ def test_dequantize_c_entry_refuses(args, says):
     refused(_lib.load().ds_dequantize_rows_i8(*args, 0), says)
 
 
-def test_desc_layout_matches_the_header():
+@pytest.mark.parametrize("name,cls", [("ds_gemm_i8_desc", _lib.GemmI8Desc), ("ds_rmsnorm_desc", _lib.RmsnormDesc)])
+def test_desc_layout_matches_the_header(name, cls):
     header = re.sub(r"/\*.*?\*/", "", open(os.path.join(REPO, "include", "dynscaler_hip.h")).read(), flags=re.S)
-    body = re.search(r"typedef struct ds_gemm_i8_desc \{(.*?)\} ds_gemm_i8_desc;", header, flags=re.S).group(1)
-    fields = [(n.strip(), t) for t, names in re.findall(r"(int(?:32|64)_t) ([^;]+);", body) for n in names.split(",")]
-    assert [(n, {C.c_int64: "int64_t", C.c_int32: "int32_t"}[t]) for n, t in _lib.GemmI8Desc._fields_] == fields
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), header, flags=re.S).group(1)
+    fields = [(n.strip(), t) for t, names in re.findall(r"(int32_t|int64_t|float) ([^;]+);", body) for n in names.split(",")]
+    assert [(n, {C.c_int64: "int64_t", C.c_int32: "int32_t", C.c_float: "float"}[t]) for n, t in cls._fields_] == fields
+    values = list(range(1, len(fields) + 1))
+    assert cls.packed(*values) == bytes(cls(*values)) and C.sizeof(cls) == len(cls.packed(*values))
