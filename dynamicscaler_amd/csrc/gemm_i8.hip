@@ -21,7 +21,7 @@ typedef f32x4 __attribute__((aligned(4))) f32x4_u;
 struct I8Args {
     const int8_t* A; const int8_t* W; const float* a_scale; const float* w_scale; const float* bias; const void* residual; void* out;
     long lda, ldw, ldr, ldc;
-    int M, N, K, epilogue, tiles_m, tiles_n;
+    int M, N, K, epilogue, tiles_m, tiles_n, group_m;
 };
 
 constexpr int BKB = 128;   // bytes (= values of k) of a K-step: 8 chunks of 16 bytes
@@ -132,6 +132,336 @@ __global__ void __launch_bounds__(256, 2) gemm_i8_any_kernel(I8Args p) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
+// M <= 16 MT: the weights are read once and that is the time.  A workgroup owns 16 columns (GEGLU: 16 values and their 16 gates); its waves
+// split K in turns of 128 bytes a row and read both operands straight from memory in fragment order (a wave's load covers 64 contiguous bytes
+// of 16 rows; W is used once, A sits in L2), then add their exact integer partial sums through LDS.  Rows past M / N repeat the last one and
+// are not stored.
+// waves of a workgroup: at most 16, and 64 KiB of partial sums
+template <int MT, bool GEGLU> struct Few {
+    static constexpr int FIT = 64 / (MT * (GEGLU ? 2 : 1)), WAVES = FIT > 16 ? 16 : FIT;
+};
+
+template <int MT, bool GEGLU>
+__global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kernel(I8Args p) {
+    constexpr int NT = GEGLU ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) i32x4 red[];      // [waves][NT][MT][64 lanes]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int l15 = lane & 15, l4 = lane >> 4;
+    const int n0 = GEGLU ? (blockIdx.x >> 1) * 64 + (blockIdx.x & 1) * 16 : blockIdx.x * 16;
+    const int8_t* w[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) w[t] = p.W + (long)min(n0 + 32 * t + l15, p.N - 1) * p.ldw;
+    const int8_t* a[MT];
+#pragma unroll
+    for (int u = 0; u < MT; ++u) a[u] = p.A + (long)min(16 * u + l15, p.M - 1) * p.lda;
+    i32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
+    const int whole = p.K / 128;
+    for (int b = wave; b < whole; b += waves) {
+        const int k = b * 128 + 16 * l4;
+        i32x4 fw[NT][2], fa[MT][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) fw[t][s] = (i32x4)*reinterpret_cast<const u32x4_u*>(w[t] + k + 64 * s);
+#pragma unroll
+            for (int u = 0; u < MT; ++u) fa[u][s] = (i32x4)*reinterpret_cast<const u32x4_u*>(a[u] + k + 64 * s);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int u = 0; u < MT; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t][s], fa[u][s], acc[t][u], 0, 0, 0);
+    }
+    if (p.K % 128 != 0 && wave == whole % waves) {
+        for (int k0 = whole * 128; k0 < p.K; k0 += 64) {
+            i32x4 fw[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) fw[t] = (i32x4)load_chunk(w[t], k0 + 16 * l4, p.K);
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+                const i32x4 fa = (i32x4)load_chunk(a[u], k0 + 16 * l4, p.K);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t], fa, acc[t][u], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) red[((wave * NT + t) * MT + u) * 64 + lane] = acc[t][u];
+    __syncthreads();
+    for (int u = wave; u < MT; u += waves) {
+        i32x4 sum[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            sum[t] = red[(t * MT + u) * 64 + lane];
+            for (int v = 1; v < waves; ++v) sum[t] += red[((v * NT + t) * MT + u) * 64 + lane];
+        }
+        const int m = 16 * u + l15;
+        if (m >= p.M) continue;
+        const float sa = p.a_scale[m];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = n0 + 4 * l4 + j;
+            if (n >= p.N) continue;
+            float v = scaled(sum[0][j], sa, p.w_scale[n], p.bias ? p.bias[n] : 0.0f);
+            int col = n;
+            if constexpr (GEGLU) {
+                v *= gelu_f(scaled(sum[1][j], sa, p.w_scale[n + 32], p.bias ? p.bias[n + 32] : 0.0f));
+                col = (blockIdx.x >> 1) * 32 + (blockIdx.x & 1) * 16 + 4 * l4 + j;
+            } else if (p.epilogue & DS_EPI_SILU) {
+                v = silu_f(v);
+            }
+            store_at(p, m, col, v + residual_at(p, m, col));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ many rows
+typedef __attribute__((address_space(3))) void lds_void;
+// LDS-DMA: lane l's 16 bytes land at dst + 16 l (dst wave-uniform); offsets past the buffer's end bring zeros
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, int8_t* dst, unsigned voff, unsigned soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)dst, 16, voff, soff, 0, 0);
+}
+constexpr unsigned OOB = 0x80000000u;    // past every buffer (all are < 2 GiB)
+
+template <int BM, int BN, int WGM, int WGN> struct I8Tile {
+    static constexpr int NT = 64 * WGM * WGN;
+    static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
+    static constexpr int LROWS = NT / 8, AR = BM / LROWS, BR = BN / LROWS;
+    static constexpr size_t STAGE = (size_t)(BM + BN) * BKB, LDS = 2 * STAGE;
+    static constexpr int PER_CU = (int)(163840 / LDS) * (NT / 64) > 16 ? 16 / (NT / 64) : (int)(163840 / LDS);
+    static_assert(BM % (16 * WGM) == 0 && WN % 64 == 0 && BM % LROWS == 0 && BN % LROWS == 0 && LROWS % 32 == 0, "tile shape");
+};
+
+// K % 16 == 0 and 16-byte aligned rows: both operands by LDS-DMA into two stages, the next K-step's pieces issued between the MFMAs of this one.
+// A stage holds BM rows of A, then BN rows of W, 128 bytes each, the 16-byte chunks XOR-swizzled through the SOURCE address so that a fragment
+// read touches every bank once.  fp16 results: the wave's W rows are dealt to its MFMA tiles so that a lane ends up with 8 consecutive columns
+// (tile t, row i <-> column 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4) and a wave stores 64 contiguous bytes of 16 rows, as it does with the
+// natural order in fp32.
+template <int BM, int BN, int WGM, int WGN, bool OUT32, bool GEGLU>
+__global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN, WGM, WGN>::PER_CU * I8Tile<BM, BN, WGM, WGN>::NT / 256)) gemm_i8_tile_kernel(I8Args p) {
+    using T = I8Tile<BM, BN, WGM, WGN>;
+    constexpr int TM = T::TM, TN = T::TN;
+    extern __shared__ __attribute__((aligned(256))) int8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    const int l15 = lane & 15, l4 = lane >> 4;
+    // workgroups that share an XCD (blockIdx % 8) take consecutive tiles; within them group_m row panels walk the columns together
+    int tile_m, tile_n;
+    {
+        const int nwg = p.tiles_m * p.tiles_n, xcd = blockIdx.x & 7, q = nwg >> 3, r = nwg & 7;
+        const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
+        const int per = p.group_m * p.tiles_n, first = (id / per) * p.group_m, in = id % per;
+        const int size = min(p.tiles_m - first, p.group_m);
+        tile_m = first + in % size;
+        tile_n = in / size;
+    }
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int rows_a = min(BM, p.M - m0), rows_w = min(BN, p.N - n0);
+    const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.A + (long)m0 * p.lda), 0, (int)((rows_a - 1) * (int)p.lda + p.K), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsW = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.W + (long)n0 * p.ldw), 0, (int)((rows_w - 1) * (int)p.ldw + p.K), 0x00020000);
+    // staging: lane -> row tid / 8 (+ LROWS per piece), physical chunk tid % 8, whose source is the chunk that the swizzle puts there
+    const int srow = tid >> 3;
+    auto swz_a = [](int row) { return (row >> 1) & 7; };
+    auto swz_w = [](int row) { return OUT32 ? (row >> 1) & 7 : ((row >> 1) & 1) | (((row >> 3) & 3) << 1); };
+    const int ca = (tid & 7) ^ swz_a(srow), cw = (tid & 7) ^ swz_w(srow);
+    unsigned va[T::AR], vw[T::BR];
+#pragma unroll
+    for (int i = 0; i < T::AR; ++i) va[i] = srow + T::LROWS * i < rows_a ? (unsigned)(srow + T::LROWS * i) * (unsigned)p.lda + 16u * ca : OOB;
+#pragma unroll
+    for (int i = 0; i < T::BR; ++i) vw[i] = srow + T::LROWS * i < rows_w ? (unsigned)(srow + T::LROWS * i) * (unsigned)p.ldw + 16u * cw : OOB;
+    const int nk = (p.K + BKB - 1) / BKB, last = p.K - (nk - 1) * BKB;      // bytes of the last K-step; chunks behind them bring zeros
+    const unsigned cut_a = 16 * ca >= last ? OOB : 0u, cut_w = 16 * cw >= last ? OOB : 0u;
+    constexpr int PIECES = T::AR + T::BR;
+    auto piece = [&](int j, int kt) {
+        int8_t* stage = smem + (kt & 1) * T::STAGE;
+        const bool tail = kt == nk - 1;
+        if (j < T::AR) dma16(rsA, stage + (T::LROWS * j + 8 * wave) * BKB, va[j] | (tail ? cut_a : 0u), (unsigned)kt * BKB);
+        else dma16(rsW, stage + (BM + T::LROWS * (j - T::AR) + 8 * wave) * BKB, vw[j - T::AR] | (tail ? cut_w : 0u), (unsigned)kt * BKB);
+    };
+    i32x4 acc[TN][TM];
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int u = 0; u < TM; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
+    // every wave's pieces have landed and every wave is through with the other stage (lgkmcnt: its fragment reads, before they are overwritten)
+    auto sync = [&]() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) piece(j, 0);
+    sync();
+    auto kstep = [&](int kt, bool more) {
+        const int8_t* sa = smem + (kt & 1) * T::STAGE + wm * T::WM * BKB;
+        const int8_t* sw = smem + (kt & 1) * T::STAGE + (BM + wn * T::WN) * BKB;
+        auto read_a = [&](int ks, int u) {
+            const int row = u * 16 + l15;
+            return *reinterpret_cast<const i32x4*>(sa + row * BKB + ((4 * ks + l4) ^ swz_a(row)) * 16);
+        };
+        auto read_w = [&](int ks, int t) {
+            const int row = OUT32 ? t * 16 + l15 : 32 * (t >> 1) + 8 * (l15 >> 2) + 4 * (t & 1) + (l15 & 3);
+            return *reinterpret_cast<const i32x4*>(sw + row * BKB + ((4 * ks + l4) ^ swz_w(row)) * 16);
+        };
+        // the short side's fragments of a 64-deep slice are held (two sets), the long side streams through a ring of three
+        constexpr bool STREAM_A = TM >= TN;
+        constexpr int L = STREAM_A ? TM : TN, S = STREAM_A ? TN : TM, NF = 2 * L, SLOTS = NF * S, SPAN = SLOTS / 2;
+        static_assert(SPAN >= PIECES, "the next K-step's pieces fit the first half of this one");
+        i32x4 held[2][S], ring[3];
+        auto read_s = [&](int ks, int t) { return STREAM_A ? read_w(ks, t) : read_a(ks, t); };
+        auto read_l = [&](int f) { return STREAM_A ? read_a(f / L, f % L) : read_w(f / L, f % L); };
+#pragma unroll
+        for (int t = 0; t < S; ++t) held[0][t] = read_s(0, t);
+        ring[0] = read_l(0);
+        ring[1] = read_l(1);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int ks = f / L, li = f % L;
+            __builtin_amdgcn_sched_barrier(0);
+            if (f + 2 < NF) ring[(f + 2) % 3] = read_l(f + 2);
+            if (ks == 0 && li < S) held[1][li] = read_s(1, li);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int si = 0; si < S; ++si) {
+                const int u = STREAM_A ? li : si, t = STREAM_A ? si : li;
+                acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(STREAM_A ? held[ks][si] : ring[f % 3], STREAM_A ? ring[f % 3] : held[ks][si], acc[t][u], 0, 0, 0);
+                const int slot = f * S + si;
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j)
+                    if (slot == ((j + 1) * SPAN) / PIECES - 1) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (more) piece(j, kt + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+        }
+        sync();
+    };
+    for (int kt = 0; kt < nk; ++kt) kstep(kt, kt + 1 < nk);
+
+    // epilogue straight from the accumulators: 8 (fp16) or 4 (fp32) consecutive columns a lane
+    constexpr int G = OUT32 ? 1 : 2, CW = 4 * G;               // tiles and columns of a lane's group
+    constexpr int GROUPS = (GEGLU ? TN / 2 : TN) / G;
+    const int mw = m0 + wm * T::WM, nw = n0 + wn * T::WN;
+    float sa[TM];
+#pragma unroll
+    for (int u = 0; u < TM; ++u) sa[u] = p.a_scale[min(mw + 16 * u + l15, p.M - 1)];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        // GEGLU: 64 columns = 32 values, 32 gates; value group g of 64-column block b, its gates 32 columns on
+        constexpr int GB = GEGLU ? 32 / (16 * G) : 1;          // groups of a 64-column block
+        const int t0 = GEGLU ? (g / GB) * 4 + (g % GB) * G : g * G;
+        const int nl = 16 * t0 + CW * l4, n = nw + nl;         // (tiles t0, t0 + 1 span 32 columns: lane l4 holds 8 l4 ... 8 l4 + 7 of them)
+        if (n >= p.N) continue;
+        float sw[CW], bw[CW], sg[CW], bg[CW];
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+            const int c = min(n + j, p.N - 1);
+            sw[j] = p.w_scale[c];
+            bw[j] = p.bias ? p.bias[c] : 0.0f;
+            if constexpr (GEGLU) {
+                sg[j] = p.w_scale[c + 32];
+                bg[j] = p.bias ? p.bias[c + 32] : 0.0f;
+            }
+        }
+        const int col = GEGLU ? (nw + 64 * (g / GB)) / 2 + (g % GB) * 16 * G + CW * l4 : n;
+        const int cols = GEGLU ? p.N / 2 : p.N;
+#pragma unroll
+        for (int u = 0; u < TM; ++u) {
+            const int m = mw + 16 * u + l15;
+            if (m >= p.M) continue;
+            float v[CW];
+#pragma unroll
+            for (int j = 0; j < CW; ++j) {
+                v[j] = scaled(acc[t0 + j / 4][u][j % 4], sa[u], sw[j], bw[j]);
+                if constexpr (GEGLU) {
+                    const float gate = scaled(acc[t0 + 2 + j / 4][u][j % 4], sa[u], sg[j], bg[j]);
+                    v[j] *= gelu_f(gate);
+                } else if (p.epilogue & DS_EPI_SILU) {
+                    v[j] = silu_f(v[j]);
+                }
+            }
+            if (col + CW <= cols) {
+                if (!GEGLU && p.residual) {
+                    const long at = (long)m * p.ldr + col;
+                    if (p.epilogue & DS_EPI_RES_F32) {
+                        const float* r = reinterpret_cast<const float*>(p.residual) + at;
+#pragma unroll
+                        for (int j = 0; j < CW; j += 4) {
+                            const f32x4 x = *reinterpret_cast<const f32x4_u*>(r + j);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[j + i] += x[i];
+                        }
+                    } else {
+                        const f16* r = reinterpret_cast<const f16*>(p.residual) + at;
+#pragma unroll
+                        for (int j = 0; j < CW; j += 4) {
+                            const f16x4 x = *reinterpret_cast<const f16x4_u*>(r + j);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[j + i] += (float)x[i];
+                        }
+                    }
+                }
+                const long at = (long)m * p.ldc + col;
+                if constexpr (OUT32) {
+                    *reinterpret_cast<f32x4_u*>(reinterpret_cast<float*>(p.out) + at) = f32x4{v[0], v[1], v[2], v[3]};
+                } else {
+                    f16x8 h;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
+                    *reinterpret_cast<f16x8_u*>(reinterpret_cast<f16*>(p.out) + at) = h;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < CW; ++j)
+                    if (col + j < cols) store_at(p, m, col + j, v[j] + residual_at(p, m, col + j));
+            }
+        }
+    }
+}
+
+template <int BM, int BN, int WGM, int WGN, bool OUT32, bool GEGLU>
+int launch_tile(I8Args p, hipStream_t st) {
+    using T = I8Tile<BM, BN, WGM, WGN>;
+    p.tiles_m = ds_cdiv(p.M, BM);
+    p.tiles_n = ds_cdiv(p.N, BN);
+    const long tiles = (long)p.tiles_m * p.tiles_n;
+    DS_CHECK_ARG(tiles * T::NT <= 0xffffffffL, "ds_gemm_i8: M %d x N %d has too many tiles for one launch", p.M, p.N);
+    p.group_m = p.tiles_n > 8 ? 8 : 1;
+    auto kernel = gemm_i8_tile_kernel<BM, BN, WGM, WGN, OUT32, GEGLU>;
+    if (T::LDS > 65536) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::LDS);
+        if (e != hipSuccess) { ds_set_error("ds_gemm_i8: %s", hipGetErrorString(e)); return DS_ELAUNCH; }
+    }
+    kernel<<<(int)tiles, T::NT, T::LDS, st>>>(p);
+    return DS_OK;
+}
+
+template <int BM, int BN, int WGM, int WGN>
+int launch_tile(const I8Args& p, hipStream_t st) {
+    const bool f32 = p.epilogue & DS_EPI_OUT_F32;
+    if (p.epilogue & DS_EPI_GEGLU) return f32 ? launch_tile<BM, BN, WGM, WGN, true, true>(p, st) : launch_tile<BM, BN, WGM, WGN, false, true>(p, st);
+    return f32 ? launch_tile<BM, BN, WGM, WGN, true, false>(p, st) : launch_tile<BM, BN, WGM, WGN, false, false>(p, st);
+}
+
+template <int MT>
+void launch_few(const I8Args& p, hipStream_t st) {
+    const bool geglu = p.epilogue & DS_EPI_GEGLU;
+    int waves = 1;                                   // a wave for every 256 bytes of K
+    while (waves < (geglu ? Few<MT, true>::WAVES : Few<MT, false>::WAVES) && waves * 256 < p.K) waves *= 2;
+    const size_t lds = (size_t)waves * MT * (geglu ? 2 : 1) * 1024;
+    if (geglu) gemm_i8_few_kernel<MT, true><<<p.N / 32, waves * 64, lds, st>>>(p);
+    else gemm_i8_few_kernel<MT, false><<<ds_cdiv(p.N, 16), waves * 64, lds, st>>>(p);
+}
+
 }  // namespace
 
 extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale, const float* w_scale, const float* bias, const void* residual,
@@ -154,14 +484,25 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
     const int osz = (d.epilogue & DS_EPI_OUT_F32) ? 4 : 2, rsz = (d.epilogue & DS_EPI_RES_F32) ? 4 : 2;
     DS_CHECK_ARG((((uintptr_t)a_scale | (uintptr_t)w_scale | (uintptr_t)bias) & 3) == 0 && ((uintptr_t)out & (osz - 1)) == 0 && ((uintptr_t)residual & (rsz - 1)) == 0,
                  "ds_gemm_i8: a pointer is not aligned to its element");
-    I8Args p{A, W, a_scale, w_scale, bias, residual, out, d.lda, d.ldw, d.ldr, d.ldc, d.M, d.N, d.K, d.epilogue, 0, 0};
+    I8Args p{A, W, a_scale, w_scale, bias, residual, out, d.lda, d.ldw, d.ldr, d.ldc, d.M, d.N, d.K, d.epilogue, 0, 0, 1};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    p.tiles_m = ds_cdiv(d.M, 128);
-    p.tiles_n = ds_cdiv(d.N, 64);
-    DS_CHECK_ARG((long)p.tiles_m * p.tiles_n <= 0xffffff, "ds_gemm_i8: M %d x N %d has too many tiles for one launch", d.M, d.N);
-    const dim3 grid(p.tiles_m * p.tiles_n);
-    if (geglu) gemm_i8_any_kernel<true><<<grid, 256, 0, st>>>(p);
-    else gemm_i8_any_kernel<false><<<grid, 256, 0, st>>>(p);
+    const bool dma = d.K > 0 && (((uintptr_t)A | (uintptr_t)W) & 15) == 0 && ((d.lda | d.ldw | d.K) & 15) == 0 && 256 * d.lda < OOB && 256 * d.ldw < OOB;
+    if (d.M <= 16) launch_few<1>(p, st);
+    else if (d.M <= 32) launch_few<2>(p, st);
+    else if (d.M <= 64) launch_few<4>(p, st);
+    else if (d.M <= 128) launch_few<8>(p, st);
+    else if (dma) {
+        const long big = (long)ds_cdiv(d.M, 256) * ds_cdiv(d.N, 256);
+        const int rc = big >= 256 && d.K >= 512 ? launch_tile<256, 256, 2, 4>(p, st) : (long)ds_cdiv(d.M, 128) * ds_cdiv(d.N, 128) >= 512 && d.K >= 512 ? launch_tile<128, 128, 2, 2>(p, st) : launch_tile<128, 64, 4, 1>(p, st);
+        if (rc != DS_OK) return rc;
+    } else {
+        p.tiles_m = ds_cdiv(d.M, 128);
+        p.tiles_n = ds_cdiv(d.N, 64);
+        DS_CHECK_ARG((long)p.tiles_m * p.tiles_n <= 0xffffff, "ds_gemm_i8: M %d x N %d has too many tiles for one launch", d.M, d.N);
+        const dim3 grid(p.tiles_m * p.tiles_n);
+        if (geglu) gemm_i8_any_kernel<true><<<grid, 256, 0, st>>>(p);
+        else gemm_i8_any_kernel<false><<<grid, 256, 0, st>>>(p);
+    }
     DS_CHECK_LAUNCH("ds_gemm_i8");
     return DS_OK;
 }
