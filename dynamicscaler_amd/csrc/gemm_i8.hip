@@ -26,14 +26,19 @@ struct I8Args {
 
 constexpr int BKB = 128;   // bytes (= values of k) of a K-step: 8 chunks of 16 bytes
 
-// 16 bytes of a row from byte `k` on, zeros behind the row's end
+// 16 bytes of a row from byte `k` on, zeros behind the row's end: the last bytes are read as the 16 that end there, and shifted down
 __device__ __forceinline__ u32x4 load_chunk(const int8_t* row, int k, int K) {
+    if (k + 16 <= K) return *reinterpret_cast<const u32x4_u*>(row + k);
     u32x4 v = {0, 0, 0, 0};
-    if (k + 16 <= K) {
-        v = *reinterpret_cast<const u32x4_u*>(row + k);
-    } else {
-        for (int j = 0; k + j < K; ++j) v[j >> 2] |= (unsigned)(uint8_t)row[k + j] << (8 * (j & 3));
+    if (k >= K) return v;
+    if (K >= 16) {
+        const u32x4 e = *reinterpret_cast<const u32x4_u*>(row + K - 16);
+        const unsigned long long lo = e[0] | (unsigned long long)e[1] << 32, hi = e[2] | (unsigned long long)e[3] << 32;
+        const int s = 8 * (k + 16 - K);          // 8 ... 120 bits
+        const unsigned long long l = s < 64 ? (lo >> s) | (hi << (64 - s)) : hi >> (s - 64), h = s < 64 ? hi >> s : 0;
+        return u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
     }
+    for (int j = 0; k + j < K; ++j) v[j >> 2] |= (unsigned)(uint8_t)row[k + j] << (8 * (j & 3));
     return v;
 }
 
@@ -53,83 +58,6 @@ __device__ __forceinline__ void store_at(const I8Args& p, int m, int n, float v)
     const long at = (long)m * p.ldc + n;
     if (p.epilogue & DS_EPI_OUT_F32) reinterpret_cast<float*>(p.out)[at] = v;
     else reinterpret_cast<f16*>(p.out)[at] = (f16)v;
-}
-
-// Any sizes, strides and alignments: 128 x 64 tiles, 4 waves of 32 x 64 (a wave's 64 columns hold whole GEGLU groups), operands through
-// registers (unaligned 16-byte global loads, byte loads in a row's last chunk) into two LDS stages, 16-byte chunks XOR-swizzled by
-// (row >> 1) & 7 so that a fragment read and a staging write each touch every bank once.
-template <bool GEGLU>
-__global__ void __launch_bounds__(256, 2) gemm_i8_any_kernel(I8Args p) {
-    constexpr int BM = 128, BN = 64;
-    __shared__ __attribute__((aligned(16))) int8_t sm[2][(BM + BN) * BKB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int m0 = (blockIdx.x / p.tiles_n) * BM, n0 = (blockIdx.x % p.tiles_n) * BN;
-    const int l15 = lane & 15, l4 = lane >> 4;
-    const int row = tid >> 3, chunk = tid & 7;      // staging: 32 rows per sweep, 8 lanes per row
-    u32x4 r[6];
-    auto load = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < 6; ++i) {
-            const int rr = row + 32 * (i < 4 ? i : i - 4);
-            const bool in = i < 4 ? m0 + rr < p.M : n0 + rr < p.N;
-            const int8_t* src = i < 4 ? p.A + (long)(m0 + rr) * p.lda : p.W + (long)(n0 + rr) * p.ldw;
-            r[i] = in ? load_chunk(src, k0 + 16 * chunk, p.K) : u32x4{0, 0, 0, 0};
-        }
-    };
-    auto store = [&](int s) {
-#pragma unroll
-        for (int i = 0; i < 6; ++i) {
-            const int rr = row + 32 * i;
-            *reinterpret_cast<u32x4*>(&sm[s][rr * BKB + (chunk ^ ((rr >> 1) & 7)) * 16]) = r[i];
-        }
-    };
-    i32x4 acc[4][2];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
-    const int nk = (p.K + BKB - 1) / BKB;
-    if (nk > 0) load(0);
-    for (int kt = 0; kt < nk; ++kt) {
-        store(kt & 1);
-        __syncthreads();       // stage kt & 1 is whole; the other one was last read before the previous barrier's successor store
-        if (kt + 1 < nk) load((kt + 1) * BKB);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            auto frag = [&](int rr) { return *reinterpret_cast<const i32x4*>(&sm[kt & 1][rr * BKB + ((4 * ks + l4) ^ ((rr >> 1) & 7)) * 16]); };
-            i32x4 a[2], w[4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) a[u] = frag(wave * 32 + u * 16 + l15);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) w[t] = frag(BM + t * 16 + l15);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t], a[u], acc[t][u], 0, 0, 0);
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int m = m0 + wave * 32 + u * 16 + l15;
-        if (m >= p.M) continue;
-        const float sa = p.a_scale[m];
-#pragma unroll
-        for (int t = 0; t < (GEGLU ? 2 : 4); ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + t * 16 + 4 * l4 + j;
-                if (n >= p.N) continue;
-                float v = scaled(acc[t][u][j], sa, p.w_scale[n], p.bias ? p.bias[n] : 0.0f);
-                int col = n;
-                if constexpr (GEGLU) {
-                    v *= gelu_f(scaled(acc[t + 2][u][j], sa, p.w_scale[n + 32], p.bias ? p.bias[n + 32] : 0.0f));
-                    col = n0 / 2 + t * 16 + 4 * l4 + j;
-                } else if (p.epilogue & DS_EPI_SILU) {
-                    v = silu_f(v);
-                }
-                store_at(p, m, col, v + residual_at(p, m, col));
-            }
-    }
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -240,12 +168,13 @@ template <int BM, int BN, int WGM, int WGN> struct I8Tile {
     static_assert(BM % (16 * WGM) == 0 && WN % 64 == 0 && BM % LROWS == 0 && BN % LROWS == 0 && LROWS % 32 == 0, "tile shape");
 };
 
-// K % 16 == 0 and 16-byte aligned rows: both operands by LDS-DMA into two stages, the next K-step's pieces issued between the MFMAs of this one.
-// A stage holds BM rows of A, then BN rows of W, 128 bytes each, the 16-byte chunks XOR-swizzled through the SOURCE address so that a fragment
+// Two LDS stages.  DMA (K % 16 == 0 and 16-byte aligned rows): both operands by LDS-DMA, the next K-step's pieces issued between the MFMAs of
+// this one.  Otherwise (any size, stride and alignment) through registers, loaded two K-steps ahead by unaligned 16-byte loads, rows past M / N
+// repeating the last one.  A stage holds BM rows of A, then BN rows of W, 128 bytes each, the 16-byte chunks XOR-swizzled through the SOURCE address so that a fragment
 // read touches every bank once.  fp16 results: the wave's W rows are dealt to its MFMA tiles so that a lane ends up with 8 consecutive columns
 // (tile t, row i <-> column 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4) and a wave stores 64 contiguous bytes of 16 rows, as it does with the
 // natural order in fp32.
-template <int BM, int BN, int WGM, int WGN, bool OUT32, bool GEGLU>
+template <int BM, int BN, int WGM, int WGN, bool DMA, bool OUT32, bool GEGLU>
 __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN, WGM, WGN>::PER_CU * I8Tile<BM, BN, WGM, WGN>::NT / 256)) gemm_i8_tile_kernel(I8Args p) {
     using T = I8Tile<BM, BN, WGM, WGN>;
     constexpr int TM = T::TM, TN = T::TN;
@@ -265,26 +194,47 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
     }
     const int m0 = tile_m * BM, n0 = tile_n * BN;
     const int rows_a = min(BM, p.M - m0), rows_w = min(BN, p.N - n0);
-    const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.A + (long)m0 * p.lda), 0, (int)((rows_a - 1) * (int)p.lda + p.K), 0x00020000);
-    const __amdgpu_buffer_rsrc_t rsW = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.W + (long)n0 * p.ldw), 0, (int)((rows_w - 1) * (int)p.ldw + p.K), 0x00020000);
     // staging: lane -> row tid / 8 (+ LROWS per piece), physical chunk tid % 8, whose source is the chunk that the swizzle puts there
     const int srow = tid >> 3;
     auto swz_a = [](int row) { return (row >> 1) & 7; };
     auto swz_w = [](int row) { return OUT32 ? (row >> 1) & 7 : ((row >> 1) & 1) | (((row >> 3) & 3) << 1); };
     const int ca = (tid & 7) ^ swz_a(srow), cw = (tid & 7) ^ swz_w(srow);
-    unsigned va[T::AR], vw[T::BR];
-#pragma unroll
-    for (int i = 0; i < T::AR; ++i) va[i] = srow + T::LROWS * i < rows_a ? (unsigned)(srow + T::LROWS * i) * (unsigned)p.lda + 16u * ca : OOB;
-#pragma unroll
-    for (int i = 0; i < T::BR; ++i) vw[i] = srow + T::LROWS * i < rows_w ? (unsigned)(srow + T::LROWS * i) * (unsigned)p.ldw + 16u * cw : OOB;
-    const int nk = (p.K + BKB - 1) / BKB, last = p.K - (nk - 1) * BKB;      // bytes of the last K-step; chunks behind them bring zeros
-    const unsigned cut_a = 16 * ca >= last ? OOB : 0u, cut_w = 16 * cw >= last ? OOB : 0u;
+    const int nk = (p.K + BKB - 1) / BKB;
     constexpr int PIECES = T::AR + T::BR;
+    // DMA: byte offsets inside the tile's rows (its operands as buffers that end with its last row), registers: addresses
+    const int8_t* a_tile = p.A + (long)m0 * p.lda;
+    const int8_t* w_tile = p.W + (long)n0 * p.ldw;
+    const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a_tile), 0, DMA ? (rows_a - 1) * (int)p.lda + p.K : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsW = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w_tile), 0, DMA ? (rows_w - 1) * (int)p.ldw + p.K : 0, 0x00020000);
+    unsigned voff[PIECES];
+    const int8_t* src[PIECES];
+    u32x4 reg[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        const bool of_a = j < T::AR;
+        const int row = srow + T::LROWS * (of_a ? j : j - T::AR), rows = of_a ? rows_a : rows_w;
+        if constexpr (DMA) voff[j] = row < rows ? (unsigned)row * (unsigned)(of_a ? p.lda : p.ldw) + 16u * (of_a ? ca : cw) : OOB;
+        else src[j] = (of_a ? a_tile : w_tile) + (long)min(row, rows - 1) * (of_a ? p.lda : p.ldw);
+    }
+    const int last = p.K - (nk - 1) * BKB;      // bytes of the last K-step; chunks behind them bring zeros
+    const unsigned cut_a = 16 * ca >= last ? OOB : 0u, cut_w = 16 * cw >= last ? OOB : 0u;
+    auto stage_row = [&](int j, int kt) { return smem + (kt & 1) * T::STAGE + (j < T::AR ? T::LROWS * j : BM + T::LROWS * (j - T::AR)) * BKB; };
     auto piece = [&](int j, int kt) {
-        int8_t* stage = smem + (kt & 1) * T::STAGE;
         const bool tail = kt == nk - 1;
-        if (j < T::AR) dma16(rsA, stage + (T::LROWS * j + 8 * wave) * BKB, va[j] | (tail ? cut_a : 0u), (unsigned)kt * BKB);
-        else dma16(rsW, stage + (BM + T::LROWS * (j - T::AR) + 8 * wave) * BKB, vw[j - T::AR] | (tail ? cut_w : 0u), (unsigned)kt * BKB);
+        dma16(j < T::AR ? rsA : rsW, stage_row(j, kt) + 8 * wave * BKB, voff[j] | (tail ? (j < T::AR ? cut_a : cut_w) : 0u), (unsigned)kt * BKB);
+    };
+    auto load_regs = [&](int kt) {
+        if (kt + 1 < nk || last == BKB) {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) reg[j] = *reinterpret_cast<const u32x4_u*>(src[j] + kt * BKB + 16 * (j < T::AR ? ca : cw));
+        } else {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) reg[j] = load_chunk(src[j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
+        }
+    };
+    auto store_regs = [&](int kt) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) *reinterpret_cast<u32x4*>(stage_row(j, kt) + srow * BKB + (tid & 7) * 16) = reg[j];
     };
     i32x4 acc[TN][TM];
 #pragma unroll
@@ -293,14 +243,25 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
         for (int u = 0; u < TM; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
     // every wave's pieces have landed and every wave is through with the other stage (lgkmcnt: its fragment reads, before they are overwritten)
     auto sync = [&]() {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    if constexpr (DMA) {
 #pragma unroll
-    for (int j = 0; j < PIECES; ++j) piece(j, 0);
+        for (int j = 0; j < PIECES; ++j) piece(j, 0);
+    } else if (nk > 0) {
+        load_regs(0);
+        store_regs(0);
+        if (nk > 1) load_regs(1);
+    }
     sync();
     auto kstep = [&](int kt, bool more) {
+        if constexpr (!DMA) {        // K-step kt + 1 into the stage that every wave has left, kt + 2 on its way
+            if (more) store_regs(kt + 1);
+            if (kt + 2 < nk) load_regs(kt + 2);
+        }
         const int8_t* sa = smem + (kt & 1) * T::STAGE + wm * T::WM * BKB;
         const int8_t* sw = smem + (kt & 1) * T::STAGE + (BM + wn * T::WN) * BKB;
         auto read_a = [&](int ks, int u) {
@@ -338,7 +299,7 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
                 for (int j = 0; j < PIECES; ++j)
                     if (slot == ((j + 1) * SPAN) / PIECES - 1) {
                         __builtin_amdgcn_sched_barrier(0);
-                        if (more) piece(j, kt + 1);
+                        if (DMA && more) piece(j, kt + 1);
                         __builtin_amdgcn_sched_barrier(0);
                     }
             }
@@ -428,7 +389,7 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
     }
 }
 
-template <int BM, int BN, int WGM, int WGN, bool OUT32, bool GEGLU>
+template <int BM, int BN, int WGM, int WGN, bool DMA, bool OUT32, bool GEGLU>
 int launch_tile(I8Args p, hipStream_t st) {
     using T = I8Tile<BM, BN, WGM, WGN>;
     p.tiles_m = ds_cdiv(p.M, BM);
@@ -436,7 +397,7 @@ int launch_tile(I8Args p, hipStream_t st) {
     const long tiles = (long)p.tiles_m * p.tiles_n;
     DS_CHECK_ARG(tiles * T::NT <= 0xffffffffL, "ds_gemm_i8: M %d x N %d has too many tiles for one launch", p.M, p.N);
     p.group_m = p.tiles_n > 8 ? 8 : 1;
-    auto kernel = gemm_i8_tile_kernel<BM, BN, WGM, WGN, OUT32, GEGLU>;
+    auto kernel = gemm_i8_tile_kernel<BM, BN, WGM, WGN, DMA, OUT32, GEGLU>;
     if (T::LDS > 65536) {
         hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::LDS);
         if (e != hipSuccess) { ds_set_error("ds_gemm_i8: %s", hipGetErrorString(e)); return DS_ELAUNCH; }
@@ -445,11 +406,11 @@ int launch_tile(I8Args p, hipStream_t st) {
     return DS_OK;
 }
 
-template <int BM, int BN, int WGM, int WGN>
+template <int BM, int BN, int WGM, int WGN, bool DMA>
 int launch_tile(const I8Args& p, hipStream_t st) {
     const bool f32 = p.epilogue & DS_EPI_OUT_F32;
-    if (p.epilogue & DS_EPI_GEGLU) return f32 ? launch_tile<BM, BN, WGM, WGN, true, true>(p, st) : launch_tile<BM, BN, WGM, WGN, false, true>(p, st);
-    return f32 ? launch_tile<BM, BN, WGM, WGN, true, false>(p, st) : launch_tile<BM, BN, WGM, WGN, false, false>(p, st);
+    if (p.epilogue & DS_EPI_GEGLU) return f32 ? launch_tile<BM, BN, WGM, WGN, DMA, true, true>(p, st) : launch_tile<BM, BN, WGM, WGN, DMA, false, true>(p, st);
+    return f32 ? launch_tile<BM, BN, WGM, WGN, DMA, true, false>(p, st) : launch_tile<BM, BN, WGM, WGN, DMA, false, false>(p, st);
 }
 
 template <int MT>
@@ -491,17 +452,18 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
     else if (d.M <= 32) launch_few<2>(p, st);
     else if (d.M <= 64) launch_few<4>(p, st);
     else if (d.M <= 128) launch_few<8>(p, st);
-    else if (dma) {
-        const long big = (long)ds_cdiv(d.M, 256) * ds_cdiv(d.N, 256);
-        const int rc = big >= 256 && d.K >= 512 ? launch_tile<256, 256, 2, 4>(p, st) : (long)ds_cdiv(d.M, 128) * ds_cdiv(d.N, 128) >= 512 && d.K >= 512 ? launch_tile<128, 128, 2, 2>(p, st) : launch_tile<128, 64, 4, 1>(p, st);
+    else {
+        auto tiles = [&](int t) { return (long)ds_cdiv(d.M, t) * ds_cdiv(d.N, t); };
+        int rc;
+        if (dma) {
+            if (tiles(256) >= 256 && d.K >= 512) rc = launch_tile<256, 256, 2, 4, true>(p, st);
+            else if (tiles(128) >= 512 && d.K >= 512) rc = launch_tile<128, 128, 2, 2, true>(p, st);
+            else rc = launch_tile<128, 64, 4, 1, true>(p, st);
+        } else {
+            if (tiles(128) >= 512) rc = launch_tile<128, 128, 2, 2, false>(p, st);
+            else rc = launch_tile<64, 64, 4, 1, false>(p, st);
+        }
         if (rc != DS_OK) return rc;
-    } else {
-        p.tiles_m = ds_cdiv(d.M, 128);
-        p.tiles_n = ds_cdiv(d.N, 64);
-        DS_CHECK_ARG((long)p.tiles_m * p.tiles_n <= 0xffffff, "ds_gemm_i8: M %d x N %d has too many tiles for one launch", d.M, d.N);
-        const dim3 grid(p.tiles_m * p.tiles_n);
-        if (geglu) gemm_i8_any_kernel<true><<<grid, 256, 0, st>>>(p);
-        else gemm_i8_any_kernel<false><<<grid, 256, 0, st>>>(p);
     }
     DS_CHECK_LAUNCH("ds_gemm_i8");
     return DS_OK;
