@@ -15,8 +15,10 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 // the same 16 bytes at any address (global memory accepts them unaligned)
 typedef u32x4 __attribute__((aligned(1))) u32x4_u;
 typedef f16x8 __attribute__((aligned(2))) f16x8_u;
-typedef f16x4 __attribute__((aligned(2))) f16x4_u;
 typedef f32x4 __attribute__((aligned(4))) f32x4_u;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 __attribute__((aligned(4))) u32x4_4;
+typedef u32x2 __attribute__((aligned(2))) u32x2_2;
 
 struct I8Args {
     const int8_t* A; const int8_t* W; const float* a_scale; const float* w_scale; const float* bias; const void* residual; void* out;
@@ -45,6 +47,24 @@ __device__ __forceinline__ u32x4 load_chunk(const int8_t* row, int k, int K) {
 __device__ __forceinline__ float silu_f(float v) { return v / (1.0f + expf(-v)); }
 __device__ __forceinline__ float gelu_f(float g) { return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f)); }
 
+// The same for fp16 results: 1 + erf(g / sqrt 2) is E(|g|) for g < 0 and 2 - E(|g|) otherwise, E(a) = erfc(a / sqrt 2) = 2^-q(a) with a polynomial
+// q of degree 8 (minimax fit on [0, 9], 8.6e-6 off, so E is within 2e-5 of itself and gelu within 2e-6 absolute -- a fortieth and less of an
+// fp16 rounding); behind 9 E < 2.3e-19 counts as zero.  12 vector instructions where erff takes ~40: the GEGLU epilogue is bound by them.
+__device__ __forceinline__ float gelu_f16(float g) {
+    const float a = fabsf(g);
+    float q = -7.463252416073374e-08f;
+    q = fmaf(q, a, 3.6557733983055757e-06f);
+    q = fmaf(q, a, -7.943754462758079e-05f);
+    q = fmaf(q, a, 0.001020048395730555f);
+    q = fmaf(q, a, -0.008750868029892445f);
+    q = fmaf(q, a, 0.054304663091897964f);
+    q = fmaf(q, a, 0.4582415223121643f);
+    q = fmaf(q, a, 1.1512949466705322f);
+    q = fmaf(q, a, -3.414401817281032e-06f);
+    const float e = a < 9.0f ? __builtin_amdgcn_exp2f(-q) : 0.0f;
+    return 0.5f * g * (g < 0.0f ? e : 2.0f - e);
+}
+
 // one output value before the residual (the accumulators of a GEGLU pair come together)
 __device__ __forceinline__ float scaled(int acc, float sa, float sw, float b) { return (float)acc * sa * sw + b; }
 
@@ -62,8 +82,8 @@ __device__ __forceinline__ void store_at(const I8Args& p, int m, int n, float v)
 
 // ------------------------------------------------------------------------------------------------ few rows
 // M <= 16 MT: the weights are read once and that is the time.  A workgroup owns 16 columns (GEGLU: 16 values and their 16 gates); its waves
-// split K in turns of 128 bytes a row and read both operands straight from memory in fragment order (a wave's load covers 64 contiguous bytes
-// of 16 rows; W is used once, A sits in L2), then add their exact integer partial sums through LDS.  Rows past M / N repeat the last one and
+// split K and read both operands straight from memory in fragment order (a wave's load covers 64 contiguous bytes of 16 rows; W is used once,
+// A sits in L2), then add their exact integer partial sums through LDS.  Rows past M / N repeat the last one and
 // are not stored.
 // waves of a workgroup: at most 16, and 64 KiB of partial sums
 template <int MT, bool GEGLU> struct Few {
@@ -72,9 +92,9 @@ template <int MT, bool GEGLU> struct Few {
 
 template <int MT, bool GEGLU>
 __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kernel(I8Args p) {
-    constexpr int NT = GEGLU ? 2 : 1;
+    constexpr int NT = GEGLU ? 2 : 1, U = MT == 1 ? 8 / NT : MT <= 3 ? 4 : 2;      // blocks of 64 bytes whose loads go out together
     extern __shared__ __attribute__((aligned(16))) i32x4 red[];      // [waves][NT][MT][64 lanes]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
     const int l15 = lane & 15, l4 = lane >> 4;
     const int n0 = GEGLU ? (blockIdx.x >> 1) * 64 + (blockIdx.x & 1) * 16 : blockIdx.x * 16;
     const int8_t* w[NT];
@@ -88,35 +108,56 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int u = 0; u < MT; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
-    const int whole = p.K / 128;
-    for (int b = wave; b < whole; b += waves) {
-        const int k = b * 128 + 16 * l4;
-        i32x4 fw[NT][2], fa[MT][2];
+    const int whole = p.K / 64, per = (whole + waves - 1) / waves;
+    const int end = min(whole, (wave + 1) * per);
+    // what the epilogue needs is on its way while the product is formed
+    const int col = GEGLU ? (blockIdx.x >> 1) * 32 + (blockIdx.x & 1) * 16 + 4 * l4 : n0 + 4 * l4, cols = GEGLU ? p.N / 2 : p.N;
+    float sw[NT][4], bw[NT][4], res[4], sa = 0.0f;
+    auto row_data = [&](int u) {
+        const int m = min(16 * u + l15, p.M - 1);
+        sa = p.a_scale[m];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int j = 0; j < 4; ++j) res[j] = residual_at(p, m, min(col + j, cols - 1));
+    };
 #pragma unroll
-            for (int t = 0; t < NT; ++t) fw[t][s] = (i32x4)*reinterpret_cast<const u32x4_u*>(w[t] + k + 64 * s);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int u = 0; u < MT; ++u) fa[u][s] = (i32x4)*reinterpret_cast<const u32x4_u*>(a[u] + k + 64 * s);
+        for (int j = 0; j < 4; ++j) {
+            const int n = min(n0 + 32 * t + 4 * l4 + j, p.N - 1);
+            sw[t][j] = p.w_scale[n];
+            bw[t][j] = p.bias ? p.bias[n] : 0.0f;
         }
+    if (wave < MT) row_data(wave);
+    for (int b = wave * per; b < end; b += U) {
+        i32x4 fw[U][NT], fa[U][MT];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < U; ++i)
+            if (b + i < end) {
+                const int k = (b + i) * 64 + 16 * l4;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) fw[i][t] = (i32x4)*reinterpret_cast<const u32x4_u*>(w[t] + k);
 #pragma unroll
-                for (int u = 0; u < MT; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t][s], fa[u][s], acc[t][u], 0, 0, 0);
-    }
-    if (p.K % 128 != 0 && wave == whole % waves) {
-        for (int k0 = whole * 128; k0 < p.K; k0 += 64) {
-            i32x4 fw[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) fw[t] = (i32x4)load_chunk(w[t], k0 + 16 * l4, p.K);
-#pragma unroll
-            for (int u = 0; u < MT; ++u) {
-                const i32x4 fa = (i32x4)load_chunk(a[u], k0 + 16 * l4, p.K);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t], fa, acc[t][u], 0, 0, 0);
+                for (int u = 0; u < MT; ++u) fa[i][u] = (i32x4)*reinterpret_cast<const u32x4_u*>(a[u] + k);
             }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (b + i < end) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int u = 0; u < MT; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i][t], fa[i][u], acc[t][u], 0, 0, 0);
+            }
+    }
+    if (p.K % 64 != 0 && wave == waves - 1) {
+        const int k = whole * 64 + 16 * l4;
+        i32x4 fw[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) fw[t] = (i32x4)load_chunk(w[t], k, p.K);
+#pragma unroll
+        for (int u = 0; u < MT; ++u) {
+            const i32x4 fa = (i32x4)load_chunk(a[u], k, p.K);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t], fa, acc[t][u], 0, 0, 0);
         }
     }
 #pragma unroll
@@ -125,28 +166,23 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
         for (int u = 0; u < MT; ++u) red[((wave * NT + t) * MT + u) * 64 + lane] = acc[t][u];
     __syncthreads();
     for (int u = wave; u < MT; u += waves) {
+        if (u != wave) row_data(u);
         i32x4 sum[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             sum[t] = red[(t * MT + u) * 64 + lane];
+#pragma unroll 4
             for (int v = 1; v < waves; ++v) sum[t] += red[((v * NT + t) * MT + u) * 64 + lane];
         }
         const int m = 16 * u + l15;
         if (m >= p.M) continue;
-        const float sa = p.a_scale[m];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int n = n0 + 4 * l4 + j;
-            if (n >= p.N) continue;
-            float v = scaled(sum[0][j], sa, p.w_scale[n], p.bias ? p.bias[n] : 0.0f);
-            int col = n;
-            if constexpr (GEGLU) {
-                v *= gelu_f(scaled(sum[1][j], sa, p.w_scale[n + 32], p.bias ? p.bias[n + 32] : 0.0f));
-                col = (blockIdx.x >> 1) * 32 + (blockIdx.x & 1) * 16 + 4 * l4 + j;
-            } else if (p.epilogue & DS_EPI_SILU) {
-                v = silu_f(v);
-            }
-            store_at(p, m, col, v + residual_at(p, m, col));
+            if (col + j >= cols) continue;
+            float v = scaled(sum[0][j], sa, sw[0][j], bw[0][j]);
+            if constexpr (GEGLU) v *= gelu_f(scaled(sum[NT - 1][j], sa, sw[NT - 1][j], bw[NT - 1][j]));
+            else if (p.epilogue & DS_EPI_SILU) v = silu_f(v);
+            store_at(p, m, col + j, p.residual ? v + res[j] : v);
         }
     }
 }
@@ -175,7 +211,7 @@ template <int BM, int BN, int WGM, int WGN> struct I8Tile {
 // (tile t, row i <-> column 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4) and a wave stores 64 contiguous bytes of 16 rows, as it does with the
 // natural order in fp32.
 template <int BM, int BN, int WGM, int WGN, bool DMA, bool OUT32, bool GEGLU>
-__global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN, WGM, WGN>::PER_CU * I8Tile<BM, BN, WGM, WGN>::NT / 256)) gemm_i8_tile_kernel(I8Args p) {
+__global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * BN > 64 * 64 ? I8Tile<BM, BN, WGM, WGN>::PER_CU * I8Tile<BM, BN, WGM, WGN>::NT / 256 : 3)) gemm_i8_tile_kernel(I8Args p) {
     using T = I8Tile<BM, BN, WGM, WGN>;
     constexpr int TM = T::TM, TN = T::TN;
     extern __shared__ __attribute__((aligned(256))) int8_t smem[];
@@ -208,7 +244,8 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
     const __amdgpu_buffer_rsrc_t rsW = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w_tile), 0, DMA ? (rows_w - 1) * (int)p.ldw + p.K : 0, 0x00020000);
     unsigned voff[PIECES];
     const int8_t* src[PIECES];
-    u32x4 reg[PIECES];
+    constexpr int D = !DMA && BM * BN <= 64 * 64 ? 2 : 1;       // K-steps held in registers on their way
+    u32x4 reg[D][PIECES];
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         const bool of_a = j < T::AR;
@@ -223,18 +260,18 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
         const bool tail = kt == nk - 1;
         dma16(j < T::AR ? rsA : rsW, stage_row(j, kt) + 8 * wave * BKB, voff[j] | (tail ? (j < T::AR ? cut_a : cut_w) : 0u), (unsigned)kt * BKB);
     };
-    auto load_regs = [&](int kt) {
+    auto load_regs = [&](int kt, int set) {
         if (kt + 1 < nk || last == BKB) {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) reg[j] = *reinterpret_cast<const u32x4_u*>(src[j] + kt * BKB + 16 * (j < T::AR ? ca : cw));
+            for (int j = 0; j < PIECES; ++j) reg[set][j] = *reinterpret_cast<const u32x4_u*>(src[j] + kt * BKB + 16 * (j < T::AR ? ca : cw));
         } else {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) reg[j] = load_chunk(src[j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
+            for (int j = 0; j < PIECES; ++j) reg[set][j] = load_chunk(src[j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
         }
     };
-    auto store_regs = [&](int kt) {
+    auto store_regs = [&](int kt, int set) {
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) *reinterpret_cast<u32x4*>(stage_row(j, kt) + srow * BKB + (tid & 7) * 16) = reg[j];
+        for (int j = 0; j < PIECES; ++j) *reinterpret_cast<u32x4*>(stage_row(j, kt) + srow * BKB + (tid & 7) * 16) = reg[set][j];
     };
     i32x4 acc[TN][TM];
 #pragma unroll
@@ -252,15 +289,45 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) piece(j, 0);
     } else if (nk > 0) {
-        load_regs(0);
-        store_regs(0);
-        if (nk > 1) load_regs(1);
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (d < nk) load_regs(d, d);
+        store_regs(0, 0);
+        if (D < nk) load_regs(D, 0);
+    }
+    // residual rows of a small wave tile: on their way while the product is formed
+    constexpr int G = OUT32 ? 1 : 2, CW = 4 * G;               // MFMA tiles and consecutive columns of a lane's group
+    constexpr int GROUPS = (GEGLU ? TN / 2 : TN) / G;
+    constexpr bool EARLY = !GEGLU && TM * TN <= 8;
+    const int mw = m0 + wm * T::WM, nw = n0 + wn * T::WN;
+    u32x4 early[EARLY ? GROUPS : 1][EARLY ? TM : 1][G];
+    auto load_residual = [&](int m, int col, u32x4* to) {
+        const long at = (long)m * p.ldr + col;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            if (p.epilogue & DS_EPI_RES_F32) {
+                to[i] = *reinterpret_cast<const u32x4_4*>(reinterpret_cast<const float*>(p.residual) + at + 4 * i);
+            } else {
+                const u32x2_2 h = *reinterpret_cast<const u32x2_2*>(reinterpret_cast<const f16*>(p.residual) + at + 4 * i);
+                to[i][0] = h[0];
+                to[i][1] = h[1];
+            }
+        }
+    };
+    if (EARLY && p.residual) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const int col = nw + 16 * g * G + CW * l4;
+#pragma unroll
+            for (int u = 0; u < TM; ++u)
+                if (col + CW <= p.N) load_residual(min(mw + 16 * u + l15, p.M - 1), col, early[g][u]);
+        }
     }
     sync();
-    auto kstep = [&](int kt, bool more) {
-        if constexpr (!DMA) {        // K-step kt + 1 into the stage that every wave has left, kt + 2 on its way
-            if (more) store_regs(kt + 1);
-            if (kt + 2 < nk) load_regs(kt + 2);
+    auto kstep = [&](int kt, bool more, int set) {
+        if constexpr (!DMA) {        // K-step kt + 1 into the stage that every wave has left, the ones behind it on their way
+            if (more) store_regs(kt + 1, set);
+            if (kt + 1 + D < nk) load_regs(kt + 1 + D, set);
         }
         const int8_t* sa = smem + (kt & 1) * T::STAGE + wm * T::WM * BKB;
         const int8_t* sw = smem + (kt & 1) * T::STAGE + (BM + wn * T::WN) * BKB;
@@ -306,12 +373,12 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
         }
         sync();
     };
-    for (int kt = 0; kt < nk; ++kt) kstep(kt, kt + 1 < nk);
+    for (int k0 = 0; k0 < nk; k0 += D)
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (k0 + d < nk) kstep(k0 + d, k0 + d + 1 < nk, (d + 1) % D);
 
     // epilogue straight from the accumulators: 8 (fp16) or 4 (fp32) consecutive columns a lane
-    constexpr int G = OUT32 ? 1 : 2, CW = 4 * G;               // tiles and columns of a lane's group
-    constexpr int GROUPS = (GEGLU ? TN / 2 : TN) / G;
-    const int mw = m0 + wm * T::WM, nw = n0 + wn * T::WN;
     float sa[TM];
 #pragma unroll
     for (int u = 0; u < TM; ++u) sa[u] = p.a_scale[min(mw + 16 * u + l15, p.M - 1)];
@@ -345,30 +412,24 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (I8Tile<BM, BN
                 v[j] = scaled(acc[t0 + j / 4][u][j % 4], sa[u], sw[j], bw[j]);
                 if constexpr (GEGLU) {
                     const float gate = scaled(acc[t0 + 2 + j / 4][u][j % 4], sa[u], sg[j], bg[j]);
-                    v[j] *= gelu_f(gate);
+                    v[j] *= OUT32 ? gelu_f(gate) : gelu_f16(gate);
                 } else if (p.epilogue & DS_EPI_SILU) {
                     v[j] = silu_f(v[j]);
                 }
             }
             if (col + CW <= cols) {
                 if (!GEGLU && p.residual) {
-                    const long at = (long)m * p.ldr + col;
-                    if (p.epilogue & DS_EPI_RES_F32) {
-                        const float* r = reinterpret_cast<const float*>(p.residual) + at;
+                    u32x4 r[G];
+                    if constexpr (EARLY) {
 #pragma unroll
-                        for (int j = 0; j < CW; j += 4) {
-                            const f32x4 x = *reinterpret_cast<const f32x4_u*>(r + j);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[j + i] += x[i];
-                        }
+                        for (int i = 0; i < G; ++i) r[i] = early[g][u][i];
                     } else {
-                        const f16* r = reinterpret_cast<const f16*>(p.residual) + at;
+                        load_residual(m, col, r);
+                    }
 #pragma unroll
-                        for (int j = 0; j < CW; j += 4) {
-                            const f16x4 x = *reinterpret_cast<const f16x4_u*>(r + j);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[j + i] += (float)x[i];
-                        }
+                    for (int j = 0; j < CW; ++j) {
+                        if (p.epilogue & DS_EPI_RES_F32) v[j] += __uint_as_float(r[j / 4][j % 4]);
+                        else v[j] += (float)__builtin_bit_cast(f16x2, (unsigned)r[j / 4][(j % 4) / 2])[j % 2];
                     }
                 }
                 const long at = (long)m * p.ldc + col;
@@ -450,7 +511,10 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
     const bool dma = d.K > 0 && (((uintptr_t)A | (uintptr_t)W) & 15) == 0 && ((d.lda | d.ldw | d.K) & 15) == 0 && 256 * d.lda < OOB && 256 * d.ldw < OOB;
     if (d.M <= 16) launch_few<1>(p, st);
     else if (d.M <= 32) launch_few<2>(p, st);
+    else if (d.M <= 48) launch_few<3>(p, st);
     else if (d.M <= 64) launch_few<4>(p, st);
+    else if (d.M <= 80) launch_few<5>(p, st);
+    else if (d.M <= 96) launch_few<6>(p, st);
     else if (d.M <= 128) launch_few<8>(p, st);
     else {
         auto tiles = [&](int t) { return (long)ds_cdiv(d.M, t) * ds_cdiv(d.N, t); };
@@ -458,7 +522,8 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
         if (dma) {
             if (tiles(256) >= 256 && d.K >= 512) rc = launch_tile<256, 256, 2, 4, true>(p, st);
             else if (tiles(128) >= 512 && d.K >= 512) rc = launch_tile<128, 128, 2, 2, true>(p, st);
-            else rc = launch_tile<128, 64, 4, 1, true>(p, st);
+            else if ((long)ds_cdiv(d.M, 128) * ds_cdiv(d.N, 64) >= 256) rc = launch_tile<128, 64, 4, 1, true>(p, st);
+            else rc = launch_tile<64, 64, 4, 1, true>(p, st);
         } else {
             if (tiles(128) >= 512) rc = launch_tile<128, 128, 2, 2, false>(p, st);
             else rc = launch_tile<64, 64, 4, 1, false>(p, st);

@@ -33,19 +33,46 @@ __device__ __forceinline__ int quantum(double t, double top, double inv) {
     return t < 0.0 ? -(int)q : (int)q;
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// The same from 32-bit forms: v = t inv carries at most five roundings of 2^-24 and |v| <= 127, so it is within 3.8e-5 of the quotient, and only
+// a fraction within 2^-14 of a half (one value in 8000) needs the 64-bit one.
+template <typename F> __device__ __forceinline__ int quantum_near(float v, F&& exactly) {
+    const float q = rintf(v);
+    int i = (int)q;
+    if (fabsf(v - q) > 0.5f - 0x1p-14f) i = exactly();
+    return i;
+}
+
+// Sum / maximum over the T lanes of a team (a power of two, at most a wave), the same bits in every lane: two quad permutes, two mirrors,
+// two swaps of 16 and 32 lanes -- no trip through LDS.
+__device__ __forceinline__ void swap16(double v, double& a, double& b) {
+    const unsigned long long u = __double_as_longlong(v);
+    const auto lo = __builtin_amdgcn_permlane16_swap((unsigned)u, (unsigned)u, false, false), hi = __builtin_amdgcn_permlane16_swap((unsigned)(u >> 32), (unsigned)(u >> 32), false, false);
+    a = __longlong_as_double(lo[0] | (unsigned long long)hi[0] << 32);
+    b = __longlong_as_double(lo[1] | (unsigned long long)hi[1] << 32);
+}
+__device__ __forceinline__ void swap32(double v, double& a, double& b) {
+    const unsigned long long u = __double_as_longlong(v);
+    const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)u, (unsigned)u, false, false), hi = __builtin_amdgcn_permlane32_swap((unsigned)(u >> 32), (unsigned)(u >> 32), false, false);
+    a = __longlong_as_double(lo[0] | (unsigned long long)hi[0] << 32);
+    b = __longlong_as_double(lo[1] | (unsigned long long)hi[1] << 32);
+}
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+    const unsigned long long u = __double_as_longlong(v);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (unsigned)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (unsigned)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __longlong_as_double(lo | (unsigned long long)hi << 32);
+}
+template <int T, typename F> __device__ __forceinline__ double team_reduce(double v, F&& op) {
+    if constexpr (T >= 2) v = op(v, dpp<0xB1>(v));        // lane ^ 1
+    if constexpr (T >= 4) v = op(v, dpp<0x4E>(v));        // lane ^ 2
+    if constexpr (T >= 8) v = op(v, dpp<0x141>(v));       // 7 - lane of 8
+    if constexpr (T >= 16) v = op(v, dpp<0x140>(v));      // 15 - lane of 16
+    double a, b;
+    if constexpr (T >= 32) { swap16(v, a, b); v = op(a, b); }
+    if constexpr (T >= 64) { swap32(v, a, b); v = op(a, b); }
     return v;
 }
-__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long u = __shfl_xor(v, o);
-        v = u > v ? u : v;
-    }
-    return v;
-}
+template <int T> __device__ __forceinline__ double team_sum(double v) { return team_reduce<T>(v, [](double a, double b) { return a + b; }); }
+template <int T> __device__ __forceinline__ double team_max(double v) { return team_reduce<T>(v, [](double a, double b) { return fmax(a, b); }); }
 
 // 8 values of a row as they lie in memory (any address that is a multiple of the element's size), as fp32 (exact for fp16), and back
 typedef f16x8 __attribute__((aligned(2))) f16x8_u;
@@ -91,8 +118,8 @@ template <> struct Chunk<int8_t> {
 // stores the same bits over the shared ones (every load of a row comes before its first store, also where sum / y lie over an input).
 // A team walks rows `grid` apart and keeps its part of gamma.
 template <typename X, typename R, typename Y, bool NORM, bool RES, int T, int V>
-__global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
-    constexpr int TEAMS = 256 / T, WAVES = T / 64;
+__global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p, int rows) {
+    constexpr int TEAMS = T > 256 ? 1 : 256 / T, WAVES = T / 64;
     constexpr bool I8 = sizeof(Y) == 1;
     __shared__ double s_sum[2][WAVES > 1 ? WAVES : 1], s_top[2][WAVES > 1 ? WAVES : 1];
     const int tid = threadIdx.x, lane = tid % T, team = tid / T;
@@ -100,14 +127,11 @@ __global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
     auto chunk = [&](int v) { return (v * T + lane) * 8; };            // where the lane's chunk v would begin: it has one if that is < C,
     auto at = [&](int v) { return min(chunk(v), C - 8); };              // and it begins here
     Chunk<float> g[V];
-    bool bad_g = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         if constexpr (NORM) {
             g[v].zero();
             if (chunk(v) < C) g[v].load(p.g + at(v));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) bad_g |= !(fabsf(g[v].at(j)) < __builtin_huge_valf());
         }
     }
     int turn = 0;
@@ -140,7 +164,7 @@ __global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
             for (int v = 0; v < V; ++v) g[v].hold();      // gamma stays in 32 bits between the rows
         }
         double sum = 0.0, top = 0.0;
-        bool bad = bad_g;
+        float topf = 0.0f, bad = 0.0f;                    // NaN or infinite where a value of the row (a gamma) is
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             if (v * T * 8 >= C) break;
@@ -157,23 +181,20 @@ __global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if constexpr (NORM) {
-                    if constexpr (I8) top = fmax(top, fabs(t_of(v, j)));
+                    if constexpr (I8) {
+                        top = fmax(top, fabs(t_of(v, j)));
+                        bad = fmaf(0.0f, g[v].at(j), bad);
+                    }
                 } else {
-                    const float a = fabsf(cx[v].at(j));
-                    bad |= !(a < __builtin_huge_valf());
-                    top = fmax(top, (double)a);
+                    topf = fmaxf(topf, fabsf(cx[v].at(j)));
+                    bad = fmaf(0.0f, cx[v].at(j), bad);
                 }
             }
         }
-        if (I8 && bad) top = __builtin_nan("");
-#pragma unroll
-        for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) {
-            if constexpr (NORM) sum += __shfl_xor(sum, o);
-            if constexpr (I8) {
-                const double u = __shfl_xor(top, o);
-                top = top < u || u != u ? u : top;           // NaN stays
-            }
-        }
+        if constexpr (!NORM) top = topf;
+        if (I8 && bad != 0.0f) top = __builtin_huge_val();     // fmax passes NaN over: an infinity stands for it from here on
+        if constexpr (NORM) sum = team_sum<(T < 64 ? T : 64)>(sum);
+        if constexpr (I8) top = team_max<(T < 64 ? T : 64)>(top);
         if constexpr (T > 64) {
             if ((tid & 63) == 0) { s_sum[turn][tid >> 6] = sum; s_top[turn][tid >> 6] = top; }
             __syncthreads();                    // two copies in turn: the next row's stores come a barrier after this row's loads
@@ -182,13 +203,14 @@ __global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) {
                 sum += s_sum[turn][w];
-                const double u = s_top[turn][w];
-                top = top < u || u != u ? u : top;
+                top = fmax(top, s_top[turn][w]);
             }
         }
         const double root = NORM ? 1.0 / sqrt(sum / C + (double)p.eps) : 1.0;
         const bool off = I8 && (!(sum < __builtin_huge_val()) || !(top < __builtin_huge_val()));
         const double inv = I8 && top > 0.0 && !off ? 127.0 / top : 0.0;
+        const bool in32 = off || top == 0.0 || (top < 1e36 && top > 1e-30);       // t and 127 / top are ordinary fp32 numbers
+        const float inv32 = in32 ? (float)inv : 0.0f;
         if (I8 && live && lane == 0) p.scale[row] = off ? __builtin_nanf("") : (float)(top * root / 127.0);
         Y* y = reinterpret_cast<Y*>(p.y) + rr * p.ldy;
         R* hs = reinterpret_cast<R*>(p.h) + rr * p.ldh;
@@ -203,14 +225,21 @@ __global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
             cy.zero();
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (I8) cy.put(j, inv > 0.0 ? quantum(t_of(v, j), top, inv) : 0);
-                else cy.set(j, t_of(v, j) * root);
+                if constexpr (I8) {
+                    float t = cx[v].at(j);
+                    if constexpr (RES) t += cr[v].at(j);
+                    if constexpr (NORM) t *= g[v].at(j);
+                    if (in32) cy.put(j, quantum_near(off ? 0.0f : t * inv32, [&] { return quantum(t_of(v, j), top, inv); }));
+                    else cy.put(j, quantum(t_of(v, j), top, inv));
+                } else {
+                    cy.set(j, t_of(v, j) * root);
+                }
             }
             if (mine) cy.store(y + at(v));
             if constexpr (RES) {
                 Chunk<R> ch;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ch.set(j, h_of(v, j));
+                for (int j = 0; j < 8; ++j) ch.set(j, cx[v].at(j) + cr[v].at(j));
                 if (mine && p.h) ch.store(hs + at(v));
             }
         }
@@ -221,40 +250,38 @@ __global__ void __launch_bounds__(256) rows_team_kernel(RowsArgs p, int rows) {
 template <typename X, typename R, typename Y, bool NORM>
 __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p) {
     __shared__ double s_sum[16];
-    __shared__ unsigned long long s_top[16];
+    __shared__ double s_top[16];
     const long row = blockIdx.x;
     const int tid = threadIdx.x;
     const X* x = reinterpret_cast<const X*>(p.x) + row * p.ldx;
     const R* r = p.r ? reinterpret_cast<const R*>(p.r) + row * p.ldr : nullptr;
     auto h_of = [&](int c) { return r ? as_f64(x[c]) + as_f64(r[c]) : as_f64(x[c]); };
     double sum = 0.0;
-    unsigned long long top = 0;       // bit patterns of non-negative doubles order like the values, infinities and NaN above them
+    double top = 0.0;
     for (int c = tid; c < p.C; c += blockDim.x) {
         const double h = h_of(c);
         sum += h * h;
-        const double t = NORM ? h * (double)p.g[c] : h;
-        const unsigned long long b = __double_as_longlong(fabs(t));
-        top = b > top ? b : top;
+        const double t = fabs(NORM ? h * (double)p.g[c] : h);
+        top = fmax(top, t < __builtin_huge_val() ? t : __builtin_huge_val());        // an infinity stands for NaN too
     }
-    sum = wave_sum(sum);
-    top = wave_max(top);
+    sum = team_sum<64>(sum);
+    top = team_max<64>(top);
     if ((tid & 63) == 0) { s_sum[tid >> 6] = sum; s_top[tid >> 6] = top; }
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
         sum += s_sum[w];
-        top = s_top[w] > top ? s_top[w] : top;
+        top = fmax(top, s_top[w]);
     }
     const double root = NORM ? 1.0 / sqrt(sum / p.C + (double)p.eps) : 1.0;
-    const double dtop = __longlong_as_double(top);
     if constexpr (sizeof(Y) == 1) {
-        const bool bad = !(sum < __builtin_huge_val()) || !(dtop < __builtin_huge_val());
-        const double inv = dtop > 0.0 && !bad ? 127.0 / dtop : 0.0;
+        const bool bad = !(sum < __builtin_huge_val()) || !(top < __builtin_huge_val());
+        const double inv = top > 0.0 && !bad ? 127.0 / top : 0.0;
         int8_t* q = reinterpret_cast<int8_t*>(p.y) + row * p.ldy;
-        if (tid == 0) p.scale[row] = bad ? __builtin_nanf("") : (float)(dtop * root / 127.0);
+        if (tid == 0) p.scale[row] = bad ? __builtin_nanf("") : (float)(top * root / 127.0);
         for (int c = tid; c < p.C; c += blockDim.x) {
             const double h = h_of(c);
-            q[c] = (int8_t)(inv > 0.0 ? quantum(NORM ? h * (double)p.g[c] : h, dtop, inv) : 0);
+            q[c] = (int8_t)(inv > 0.0 ? quantum(NORM ? h * (double)p.g[c] : h, top, inv) : 0);
             if constexpr (NORM) {
                 if (p.h) reinterpret_cast<R*>(p.h)[row * p.ldh + c] = (R)h;
             }
@@ -269,26 +296,48 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p) {
     }
 }
 
-// Teams of 1 << shift lanes per row, 8 values per lane and turn.
+// The chunks of 8 values of all rows in one sequence, `span` of them a workgroup (per_row of them a row; magic: i / per_row = i * magic >> 40 for
+// i < per_row + span, both < 2^16): every lane has work whatever the row's length.  C >= 8; a row's last chunk ends at the row's end.
 template <typename Y>
-__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C, int shift) {
-    const long row = (long)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
-    if (row >= rows) return;
-    const int lane = threadIdx.x & ((1 << shift) - 1);
-    const float s = scale[row];
-    const int8_t* src = q + row * ldq;
-    Y* dst = y + row * ldy;
-    for (int c = lane * 8; c < C; c += 8 << shift) {
-        if (c + 8 <= C) {
-            const u32x2 v = *reinterpret_cast<const u32x2_u*>(src + c);
-            Chunk<Y> cy;
+__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C,
+                                                      unsigned per_row, unsigned long long magic, int span) {
+    const unsigned long long first = (unsigned long long)blockIdx.x * span;
+    const long row0 = first / per_row;
+    const unsigned in0 = (unsigned)(first - row0 * per_row);
+#pragma unroll 4
+    for (int k = threadIdx.x; k < span; k += 256) {
+        const unsigned i = in0 + k, r = (unsigned)((i * magic) >> 40);
+        const long row = row0 + r;
+        if (row >= rows) break;
+        const int c = min((int)(i - r * per_row) * 8, C - 8);
+        const float s = scale[row];
+        const u32x2 v = *reinterpret_cast<const u32x2_u*>(q + row * ldq + c);
+        Chunk<Y> cy;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) cy.set(j, (float)((int)(v[j >> 2] << (24 - 8 * (j & 3))) >> 24) * s);
-            cy.store(dst + c);
-        } else {
-            for (int j = c; j < C; ++j) dst[j] = (Y)((float)src[j] * s);
-        }
+        for (int j = 0; j < 8; ++j) cy.set(j, (float)((int)(v[j >> 2] << (24 - 8 * (j & 3))) >> 24) * s);
+        cy.store(y + row * ldy + c);
     }
+}
+
+// ... and value by value: rows of less than 8 values, or of more chunks than `magic` takes
+template <typename Y>
+__global__ void __launch_bounds__(256) dequant_any_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int C) {
+    const long row = blockIdx.x;
+    const float s = scale[row];
+    for (int c = threadIdx.x; c < C; c += 256) y[row * ldy + c] = (Y)((float)q[row * ldq + c] * s);
+}
+
+template <typename Y>
+void launch_dequant(const int8_t* q, long ldq, const float* scale, Y* y, long ldy, int rows, int C, hipStream_t st) {
+    const unsigned per_row = ds_cdiv(C, 8);
+    const long chunks = (long)per_row * rows;
+    const int span = chunks >= 1024 * 1024 ? 1024 : 256;        // four chunks a lane once they fill the chip
+    if (C < 8 || per_row + span >= 65536 || ds_cdiv(chunks, span) > 0xffffff) {
+        dequant_any_kernel<Y><<<rows, 256, 0, st>>>(q, ldq, scale, y, ldy, C);
+        return;
+    }
+    const unsigned long long magic = ((1ull << 40) + per_row - 1) / per_row;
+    dequant_kernel<Y><<<ds_cdiv(chunks, span), 256, 0, st>>>(q, ldq, scale, y, ldy, rows, C, per_row, magic, span);
 }
 
 bool rows_dtype(int t) { return t == DS_F16 || t == DS_F32; }
@@ -296,16 +345,26 @@ bool aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == DS_I8 
 
 template <typename X, typename R, typename Y, bool NORM, bool RES>
 void launch_rows(const RowsArgs& p, int rows, hipStream_t st) {
-    // the smallest team whose four chunks a lane hold the row; teams walk several rows once the chip is full (16 waves a CU)
-    constexpr int V = 4, FULL = 256 * 4;
-    auto grid = [&](int teams) { const int n = ds_cdiv(rows, teams); return n < FULL ? n : FULL; };
+    // the smallest team whose four chunks a lane hold the row; a norm's teams walk several rows, with gamma in registers, once the chip is
+    // full (16 waves a CU)
+    constexpr int V = 4;
+    auto grid = [&](int teams) { const int n = ds_cdiv(rows, teams); return NORM && n > 256 * 4 ? 256 * 4 : n; };
     if (p.C < 8) rows_long_kernel<X, R, Y, NORM><<<rows, 64, 0, st>>>(p);
     else if (p.C <= 8 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 8, V><<<grid(32), 256, 0, st>>>(p, rows);
     else if (p.C <= 16 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 16, V><<<grid(16), 256, 0, st>>>(p, rows);
     else if (p.C <= 32 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 32, V><<<grid(8), 256, 0, st>>>(p, rows);
     else if (p.C <= 64 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 64, V><<<grid(4), 256, 0, st>>>(p, rows);
     else if (p.C <= 256 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 256, V><<<grid(1), 256, 0, st>>>(p, rows);
-    else rows_long_kernel<X, R, Y, NORM><<<rows, 1024, 0, st>>>(p);
+    else if (p.C <= 512 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 512, V><<<grid(1), 512, 0, st>>>(p, rows);
+    else {
+        if constexpr (!NORM) {         // (a norm's registers do not fit 1024 threads)
+            if (p.C <= 1024 * 8 * V) {
+                rows_team_kernel<X, R, Y, NORM, RES, 1024, V><<<grid(1), 1024, 0, st>>>(p, rows);
+                return;
+            }
+        }
+        rows_long_kernel<X, R, Y, NORM><<<rows, 1024, 0, st>>>(p);
+    }
 }
 
 template <typename X, typename R, bool RES>
@@ -372,11 +431,8 @@ extern "C" int ds_dequantize_rows_i8(const int8_t* q, int64_t ldq, const float* 
     DS_CHECK_ARG(ldq >= C && ldy >= C, "ds_dequantize_rows_i8: a row stride is shorter than C %d", C);
     DS_CHECK_ARG(aligned(y, y_dtype) && aligned(scale, DS_F32), "ds_dequantize_rows_i8: a pointer is not aligned to its element");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    int shift = 3;                 // the smallest team that holds the row in one turn, at most a workgroup
-    while (shift < 8 && (8 << shift) < C) ++shift;
-    const int grid = ds_cdiv(rows, 256 >> shift);
-    if (y_dtype == DS_F32) dequant_kernel<float><<<grid, 256, 0, st>>>(q, ldq, scale, (float*)y, ldy, rows, C, shift);
-    else dequant_kernel<f16><<<grid, 256, 0, st>>>(q, ldq, scale, (f16*)y, ldy, rows, C, shift);
+    if (y_dtype == DS_F32) launch_dequant<float>(q, ldq, scale, (float*)y, ldy, rows, C, st);
+    else launch_dequant<f16>(q, ldq, scale, (f16*)y, ldy, rows, C, st);
     DS_CHECK_LAUNCH("ds_dequantize_rows_i8");
     return DS_OK;
 }

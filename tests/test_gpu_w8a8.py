@@ -5,7 +5,8 @@ Tolerances.  H(t) = half a step of a rounding to t (relative): fp16 2^-11, fp32 
             rounding of the result (H32 (|p| + |b|)), the residual one more: 5 H32 (|p| + |b| + |r|) in all, then H(out) |out|.
             SiLU: slope <= 1.1, and x / (1 + e^-x) itself: exp 2 ulp (4 H32), sum, quotient: 8 H32 |silu|.  GEGLU: value * gelu(gate): the
             errors of value and gate (slope <= 1.13) are carried, 1 + erf is off by at most 8 H32 absolute, hence gelu by 4 H32 |gate|, and
-            three products: 4 H32 |result|.
+            three products: 4 H32 |result|.  With an fp16 result gelu comes from a fit of erfc that is within 1.6e-5 of it (found on 200 000 points,
+            8.6e-6 ln 2 by the fit and its 32-bit evaluation), the 2^-q within 2e-5: 2e-5 |gate| / 2 erfc(|gate| / sqrt 2) more.
   8 bits    q has to be EQUAL: the kernel rounds the exact quotient.  scale: one rounding of a 64-bit value, H32, doubled for slack in sums.
   norm y    h, root, gamma: at most five fp32 roundings (5 H32) before H(out).
   sum       H32 + H(out).
@@ -41,7 +42,7 @@ def normal(shape, seed, dtype=F32, scale=1.0):
     return (torch.randn(shape, generator=gen(seed)) * scale).to(dtype)
 
 
-def product_ref(a, w, sa, sw, bias, residual, act):
+def product_ref(a, w, sa, sw, bias, residual, act, out=F16):
     """(result, tolerance before the output's rounding) in 64 bits."""
     p = (a.double() @ w.double().t()) * sa.double()[:, None] * sw.double()
     b = torch.zeros_like(p) if bias is None else bias.double().expand_as(p)
@@ -56,7 +57,8 @@ def product_ref(a, w, sa, sw, bias, residual, act):
         x, g, ex, eg = vv[:, :, 0], vv[:, :, 1], ee[:, :, 0], ee[:, :, 1]
         gelu = 0.5 * g * torch.erfc(-g / math.sqrt(2.0))
         v = (x * gelu).reshape(m, n // 2)
-        e = (ex * gelu.abs() + x.abs() * (1.13 * eg + 4 * H32 * g.abs()) + ex * 1.13 * eg).reshape(m, n // 2) + 4 * H32 * v.abs()
+        fit = 2e-5 * g.abs() / 2 * torch.erfc(g.abs() / math.sqrt(2.0)) if out == F16 else 0.0
+        e = (ex * gelu.abs() + x.abs() * (1.13 * eg + 4 * H32 * g.abs() + fit) + ex * 1.13 * eg).reshape(m, n // 2) + 4 * H32 * v.abs()
     if residual is not None:
         r = residual.double()
         v, e = v + r, e + 2 * H32 * (v.abs() + r.abs())
@@ -111,7 +113,7 @@ def test_product(m, n, k, out_dtype, residual):
 def test_product_activations(m, n, k, act, out_dtype, bias):
     c = product_case(m, n, k, 7 * m + n + k, bias=bias, act=act)
     got = run_product(c, act=act, out_dtype=out_dtype)
-    close(got, *product_ref(*c, act), out_dtype)
+    close(got, *product_ref(*c, act, out_dtype), out_dtype)
 
 
 @pytest.mark.parametrize("m,n,k", [(4, 40, 131071), (130, 70, 131071), (260, 256, 131056)])
