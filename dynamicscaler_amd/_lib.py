@@ -5,7 +5,6 @@ raises at import of the first op (HipLibraryMissing), loudly.
 """
 import ctypes as C
 import os
-import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # The product loads the in-tree library.  DS_HIP_LIBRARY names a diagnostic build of the same ABI instead (tests/hazard_probe.py,
@@ -40,13 +39,11 @@ class GemmDesc(C.Structure):
 
 class GemmI8Desc(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("lda", "ldw", "ldc", "ldr")] + [(n, C.c_int32) for n in ("M", "N", "K", "epilogue")]
-    packed = struct.Struct("=4q4i").pack      # the same bytes from Python numbers, for `ops` (a third of a Structure's time)
 
 
 class RmsnormDesc(C.Structure):
     _fields_ = ([(n, C.c_int64) for n in ("ldx", "ldr", "lds", "ldy")] + [(n, C.c_int32) for n in ("rows", "C", "x_dtype", "r_dtype", "y_dtype")]
                 + [("eps", C.c_float)])
-    packed = struct.Struct("=4q5if").pack
 
 
 class UNetConfig(C.Structure):
@@ -119,8 +116,8 @@ SIGNATURES = {
     "ds_clip_preprocess": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "ds_patchify": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "ds_cast_to_f16": (_i, [_vp, _i, _vp, _sz, _vp]),
-    "ds_gemm_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "ds_rmsnorm_rows": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ds_gemm_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _pp(GemmI8Desc), _vp]),
+    "ds_rmsnorm_rows": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _pp(RmsnormDesc), _vp]),
     "ds_quantize_rows_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i, _i, _vp]),
     "ds_dequantize_rows_i8": (_i, [_vp, _i64, _vp, _vp, _i, _i64, _i, _i, _vp]),
     "ds_wide_lo_scale": (_f, []),
@@ -191,6 +188,24 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_w8a8 = None
+
+
+def load_w8a8():
+    """The W8A8 operators' tensor front end (csrc/w8a8_torch.cpp), bound to the entries of the loaded library."""
+    global _w8a8
+    if _w8a8 is None:
+        lib = load()
+        try:
+            from . import _w8a8 as front
+        except ImportError as e:
+            raise HipLibraryMissing(f"cannot load {os.path.join(HERE, '_w8a8.so')}: build it with `python -m dynamicscaler_amd.build` ({e})") from e
+        front.bind(DsError, *(C.cast(f, C.c_void_p).value for f in (lib.ds_gemm_i8, lib.ds_rmsnorm_rows, lib.ds_quantize_rows_i8, lib.ds_dequantize_rows_i8,
+                                                                  lib.ds_last_error)))
+        _w8a8 = front
+    return _w8a8
 
 
 DIAG_LIB = os.path.join(HERE, "libdynscaler_diag.so")

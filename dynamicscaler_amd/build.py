@@ -99,6 +99,27 @@ def build(force=False, verbose=True, variant=None):
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    if variant is None:
+        build_torch(verbose)
+    return lib
+
+
+def build_torch(verbose=True):
+    """_w8a8.so (csrc/w8a8_torch.cpp): the tensor front end of the W8A8 operators, a CPython extension against the installed torch."""
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    src = os.path.join(CSRC, "w8a8_torch.cpp")
+    lib = os.path.join(HERE, "_w8a8.so")
+    if _newer([src, os.path.join(HERE, "..", "include", "dynscaler_hip.h")], lib):
+        cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DUSE_ROCM=1", "-D__HIP_PLATFORM_AMD__=1"]
+               + ["-I" + d for d in include_paths() + [sysconfig.get_paths()["include"], "/opt/rocm/include"]] + [src, "-o", lib]
+               + ["-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"])
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose and (r.stdout or r.stderr):
+            sys.stderr.write(r.stdout + r.stderr)
+        if r.returncode != 0:
+            raise RuntimeError("g++ failed: " + " ".join(cmd))
     return lib
 
 

@@ -88,11 +88,12 @@ __device__ __forceinline__ void store_at(const I8Args& p, int m, int n, float v)
 // waves of a workgroup: at most 16, and 64 KiB of partial sums
 template <int MT, bool GEGLU> struct Few {
     static constexpr int FIT = 64 / (MT * (GEGLU ? 2 : 1)), WAVES = FIT > 16 ? 16 : FIT;
+    static constexpr int U = MT == 1 ? (GEGLU ? 4 : 8) : MT <= 3 ? 4 : 2;      // blocks of 64 bytes whose loads a wave sends out together
 };
 
 template <int MT, bool GEGLU>
 __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kernel(I8Args p) {
-    constexpr int NT = GEGLU ? 2 : 1, U = MT == 1 ? 8 / NT : MT <= 3 ? 4 : 2;      // blocks of 64 bytes whose loads go out together
+    constexpr int NT = GEGLU ? 2 : 1, U = Few<MT, GEGLU>::U;
     extern __shared__ __attribute__((aligned(16))) i32x4 red[];      // [waves][NT][MT][64 lanes]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
     const int l15 = lane & 15, l4 = lane >> 4;
@@ -112,12 +113,19 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
     const int end = min(whole, (wave + 1) * per);
     // what the epilogue needs is on its way while the product is formed
     const int col = GEGLU ? (blockIdx.x >> 1) * 32 + (blockIdx.x & 1) * 16 + 4 * l4 : n0 + 4 * l4, cols = GEGLU ? p.N / 2 : p.N;
-    float sw[NT][4], bw[NT][4], res[4], sa = 0.0f;
+    float sw[NT][4], bw[NT][4], sa = 0.0f;
+    unsigned res[4];                     // the residual's bits as they came: a conversion here would wait for them
+    const bool res32 = p.epilogue & DS_EPI_RES_F32;
     auto row_data = [&](int u) {
         const int m = min(16 * u + l15, p.M - 1);
         sa = p.a_scale[m];
+        if (p.residual && res32) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) res[j] = residual_at(p, m, min(col + j, cols - 1));
+            for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const unsigned*>(p.residual)[(long)m * p.ldr + min(col + j, cols - 1)];
+        } else if (p.residual) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const uint16_t*>(p.residual)[(long)m * p.ldr + min(col + j, cols - 1)];
+        }
     };
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -182,7 +190,8 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
             float v = scaled(sum[0][j], sa, sw[0][j], bw[0][j]);
             if constexpr (GEGLU) v *= gelu_f(scaled(sum[NT - 1][j], sa, sw[NT - 1][j], bw[NT - 1][j]));
             else if (p.epilogue & DS_EPI_SILU) v = silu_f(v);
-            store_at(p, m, col + j, p.residual ? v + res[j] : v);
+            if (p.residual) v += res32 ? __uint_as_float(res[j]) : (float)__builtin_bit_cast(f16, (uint16_t)res[j]);
+            store_at(p, m, col + j, v);
         }
     }
 }
@@ -477,8 +486,10 @@ int launch_tile(const I8Args& p, hipStream_t st) {
 template <int MT>
 void launch_few(const I8Args& p, hipStream_t st) {
     const bool geglu = p.epilogue & DS_EPI_GEGLU;
-    int waves = 1;                                   // a wave for every 256 bytes of K
-    while (waves < (geglu ? Few<MT, true>::WAVES : Few<MT, false>::WAVES) && waves * 256 < p.K) waves *= 2;
+    // as many waves as let each have all its loads in flight at once
+    const int most = geglu ? Few<MT, true>::WAVES : Few<MT, false>::WAVES, batch = 64 * (geglu ? Few<MT, true>::U : Few<MT, false>::U);
+    int waves = 1;
+    while (waves * 2 <= most && waves * batch < p.K) waves *= 2;
     const size_t lds = (size_t)waves * MT * (geglu ? 2 : 1) * 1024;
     if (geglu) gemm_i8_few_kernel<MT, true><<<p.N / 32, waves * 64, lds, st>>>(p);
     else gemm_i8_few_kernel<MT, false><<<ds_cdiv(p.N, 16), waves * 64, lds, st>>>(p);

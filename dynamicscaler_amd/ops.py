@@ -9,8 +9,8 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import (DS_F16, DS_F32, DS_I8, DS_A_DENSE, DS_A_CONV3, DS_A_TCONV, DS_EPI_GEGLU, DS_EPI_SILU,
-                   DS_EPI_OUT_F32, DS_EPI_RES_F32, DS_MAX_WINDOWS, RingGeom, GemmDesc, GemmI8Desc, RmsnormDesc, check)
+from ._lib import (DS_F16, DS_F32, DS_A_DENSE, DS_A_CONV3, DS_A_TCONV, DS_EPI_GEGLU, DS_EPI_SILU,
+                   DS_EPI_OUT_F32, DS_EPI_RES_F32, DS_MAX_WINDOWS, RingGeom, GemmDesc, check)
 
 _DT = {torch.float16: DS_F16, torch.float32: DS_F32}
 
@@ -546,57 +546,17 @@ def temporal_attention(q, k, v, out, *, nseq_batches, T, hw, heads, ldq, ldk, ld
 
 
 # ------------------------------------------------------------------------------------------------ W8A8
-# A call on a few rows is over on the GPU before the host has made the next one, so the checks below take the short way for what nearly
-# every call passes (contiguous tensors of the right type and shape) and explain themselves only when that fails.
-_ROWS = (torch.float16, torch.float32)
-_INT8 = (torch.int8,)
-_F16, _F32, _I8 = torch.float16, torch.float32, torch.int8
+# The checks, the outputs' allocation and the call are C++ (csrc/w8a8_torch.cpp): on a few rows the host's share of a call is longer than the
+# kernel.  Every function takes 2-D tensors with contiguous columns and any row stride that keeps rows apart, all on the current device, and
+# raises DsError for anything else.
+_W8A8 = None
 
 
-def _rows_of(t, what, dtypes, rows=None, cols=None):
-    """(rows, cols, row stride) of a 2-D tensor with unit column stride and rows that do not overlap."""
-    shape = t.shape
-    if t.dtype in dtypes and len(shape) == 2 and t.is_contiguous():
-        m, n = shape
-        if (rows is None or m == rows) and (cols is None or n == cols):
-            return m, n, n
-    if t.dtype not in dtypes:
-        raise _lib.DsError(f"{what}: {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
-    if t.dim() != 2:
-        raise _lib.DsError(f"{what}: has to be [rows, columns], got {tuple(shape)}")
-    (m, n), (ld, step) = shape, t.stride()
-    if (rows is not None and m != rows) or (cols is not None and n != cols):
-        raise _lib.DsError(f"{what}: is {m} x {n}, expected {m if rows is None else rows} x {n if cols is None else cols}")
-    if n > 1 and step != 1:
-        raise _lib.DsError(f"{what}: the columns of a row have to be contiguous (strides {ld}, {step})")
-    if m <= 1:
-        ld = n
-    elif ld < n:
-        raise _lib.DsError(f"{what}: rows overlap (row stride {ld}, {n} columns)")
-    return m, n, ld
-
-
-def _vector_of(t, what, n):
-    if t.dtype is not _F32 or t.shape != (n,) or not t.is_contiguous():
-        raise _lib.DsError(f"{what}: has to be a contiguous fp32 vector of {n} values, got {t.dtype} {tuple(t.shape)}")
-
-
-def _stream_on(stream, first, *others):
-    """The stream of a call on these tensors: the current one of their device, which has to be the current device."""
-    dev = first.get_device()
-    if dev < 0:
-        raise _lib.DsError(f"tensors are on {first.device}; the DynamicScaler hot path has no CPU fallback")
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise _lib.DsError(f"tensors on {first.device} and {t.device} in one call")
-    if dev != torch._C._cuda_getDevice():
-        raise _lib.DsError(f"tensors are on {first.device}, the current device is cuda:{torch.cuda.current_device()}: call under torch.cuda.device({dev})")
-    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream
-
-
-def _rows_dtype(what, dtype):
-    if dtype not in _ROWS:
-        raise _lib.DsError(f"{what} {dtype} is not torch.float16 or torch.float32")
+def _w8a8():
+    global _W8A8
+    if _W8A8 is None:
+        _W8A8 = _lib.load_w8a8()
+    return _W8A8
 
 
 def gemm_i8(A, W, a_scale, w_scale, bias=None, residual=None, *, out=None, out_dtype=torch.float16, epilogue=0, stream=None):
@@ -604,119 +564,38 @@ def gemm_i8(A, W, a_scale, w_scale, bias=None, residual=None, *, out=None, out_d
     (K <= 131071: the sums are exact), fp32 scales per row of A and of W and fp32 bias, fp16 / fp32 residual and out.  epilogue:
     DS_EPI_SILU or DS_EPI_GEGLU (N % 64 == 0, W's rows and the bias in 32-row groups of values and gates as for `gemm`; N / 2 output
     columns; no residual).  Any sizes, row strides and alignments; `residual` may be `out` itself."""
-    M, K, lda = _rows_of(A, "gemm_i8(A)", _INT8)
-    N, _, ldw = _rows_of(W, "gemm_i8(W)", _INT8, None, K)
-    _vector_of(a_scale, "gemm_i8(a_scale)", M)
-    _vector_of(w_scale, "gemm_i8(w_scale)", N)
-    if bias is not None:
-        _vector_of(bias, "gemm_i8(bias)", N)
-    cols = N // 2 if epilogue & DS_EPI_GEGLU else N
-    if out is None:
-        _rows_dtype("gemm_i8: out_dtype", out_dtype)
-        out, ldc = A.new_empty((M, cols), dtype=out_dtype), cols
-    else:
-        ldc, out_dtype = _rows_of(out, "gemm_i8(out)", _ROWS, M, cols)[2], out.dtype
-    flags = epilogue | DS_EPI_OUT_F32 if out_dtype is _F32 else epilogue
-    ldr = 0
-    if residual is not None:
-        ldr = _rows_of(residual, "gemm_i8(residual)", _ROWS, M, cols)[2]
-        if residual.dtype is _F32:
-            flags |= DS_EPI_RES_F32
-    st = _stream_on(stream, A, W, a_scale, w_scale, bias, residual, out)
-    args = (A.data_ptr(), W.data_ptr(), a_scale.data_ptr(), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
-            0 if residual is None else residual.data_ptr(), out.data_ptr(), GemmI8Desc.packed(lda, ldw, ldc, ldr, M, N, K, flags), st)
+    front = _W8A8 or _w8a8()
     if _timing_hook is None:
-        check(_lib.load().ds_gemm_i8(*args), "ds_gemm_i8")
-    else:
-        _timing_hook("gemm_i8", 2.0 * M * N * K, lambda: check(_lib.load().ds_gemm_i8(*args), "ds_gemm_i8"),
-                     (DS_A_DENSE, M, N, K, flags, int(residual is not None)))
-    return out
-
-
-def _rmsnorm(what, x, gamma, eps, residual, sum_out, y, scale, y_dtype, stream):
-    rows, Cch, ldx = _rows_of(x, what + "(x)", _ROWS)
-    if Cch < 1:
-        raise _lib.DsError(f"{what}: rows without values")
-    _vector_of(gamma, what + "(gamma)", Cch)
-    ldr = lds = r_type = r_ptr = s_ptr = 0
-    if residual is not None:
-        ldr, r_dtype = _rows_of(residual, what + "(residual)", _ROWS, rows, Cch)[2], residual.dtype
-        r_type = DS_F32 if r_dtype is _F32 else DS_F16
-        if sum_out is None:
-            sum_out, lds = x.new_empty((rows, Cch), dtype=r_dtype), Cch
-        else:
-            lds = _rows_of(sum_out, what + "(sum_out)", (r_dtype,), rows, Cch)[2]
-        r_ptr, s_ptr = residual.data_ptr(), sum_out.data_ptr()
-    elif sum_out is not None:
-        raise _lib.DsError(f"{what}: sum_out without a residual")
-    if y is None:
-        y, ldy = x.new_empty((rows, Cch), dtype=y_dtype), Cch
-    else:
-        ldy, y_dtype = _rows_of(y, what + "(out)", _INT8 if y_dtype is _I8 else _ROWS, rows, Cch)[2], y.dtype
-    s_out = 0
-    if y_dtype is _I8:
-        if scale is None:
-            scale = x.new_empty((rows,), dtype=_F32)
-        else:
-            _vector_of(scale, what + "(scale)", rows)
-        s_out = scale.data_ptr()
-    st = _stream_on(stream, x, gamma, residual, sum_out, y, scale)
-    check(_lib.load().ds_rmsnorm_rows(x.data_ptr(), r_ptr, gamma.data_ptr(), s_ptr, y.data_ptr(), s_out, RmsnormDesc.packed(
-        ldx, ldr, lds, ldy, rows, Cch, DS_F32 if x.dtype is _F32 else DS_F16, r_type,
-        DS_I8 if y_dtype is _I8 else DS_F32 if y_dtype is _F32 else DS_F16, eps), st), "ds_rmsnorm_rows")
-    return y, scale, sum_out
+        return front.gemm_i8(A, W, a_scale, w_scale, bias, residual, out, out_dtype, epilogue, stream)
+    made = []
+    (M, K), N = A.shape, W.shape[0]
+    _timing_hook("gemm_i8", 2.0 * M * N * K, lambda: made.append(front.gemm_i8(A, W, a_scale, w_scale, bias, residual, out, out_dtype, epilogue, stream)),
+                 (DS_A_DENSE, M, N, K, epilogue, int(residual is not None)))
+    return made[-1]
 
 
 def rmsnorm(x, gamma, eps=1e-6, residual=None, *, sum_out=None, out=None, out_dtype=torch.float16, stream=None):
     """(y, h) with h = x + residual and y = h * gamma / sqrt(mean(h^2) + eps) over each row; h in the residual's type (None without a
-    residual; the norm reads it unrounded).  x and residual fp16 / fp32 rows of any stride, gamma fp32.  sum_out may be the residual
-    itself, out may be x."""
-    _rows_dtype("rmsnorm: out_dtype", out_dtype)
-    y, _, h = _rmsnorm("rmsnorm", x, gamma, eps, residual, sum_out, out, None, out_dtype, stream)
+    residual; the norm reads it unrounded).  x and residual fp16 / fp32, gamma fp32.  sum_out may be the residual itself, out may be x."""
+    y, _, h = (_W8A8 or _w8a8()).rmsnorm("rmsnorm", False, x, gamma, eps, residual, sum_out, out, out_dtype, None, stream)
     return y, h
 
 
 def rmsnorm_i8(x, gamma, eps=1e-6, residual=None, *, sum_out=None, out=None, scale=None, stream=None):
     """(q, scale, h): `rmsnorm` with an 8-bit result, q = rint(127 y / max|y|) (exactly, halves to even) and scale = max|y| / 127 of
     each row -- the A and a_scale of `gemm_i8`.  A row of zeros has scale 0, a row with a NaN or an infinity scale NaN; their q is 0."""
-    return _rmsnorm("rmsnorm_i8", x, gamma, eps, residual, sum_out, out, scale, _I8, stream)
+    return (_W8A8 or _w8a8()).rmsnorm("rmsnorm_i8", True, x, gamma, eps, residual, sum_out, out, None, scale, stream)
 
 
 def quantize_rows_i8(x, *, out=None, scale=None, stream=None):
     """(q, scale): q = rint(127 x / max|x|) (exactly, halves to even), scale = max|x| / 127 of each fp16 / fp32 row; zeros and non-finite
     rows as in `rmsnorm_i8`.  Activations without a norm in front, or weights [N, K] -> the W and w_scale of `gemm_i8`."""
-    rows, Cch, ldx = _rows_of(x, "quantize_rows_i8(x)", _ROWS)
-    if Cch < 1:
-        raise _lib.DsError("quantize_rows_i8: rows without values")
-    if out is None:
-        out, ldq = x.new_empty((rows, Cch), dtype=_I8), Cch
-    else:
-        ldq = _rows_of(out, "quantize_rows_i8(out)", _INT8, rows, Cch)[2]
-    if scale is None:
-        scale = x.new_empty((rows,), dtype=_F32)
-    else:
-        _vector_of(scale, "quantize_rows_i8(scale)", rows)
-    st = _stream_on(stream, x, out, scale)
-    check(_lib.load().ds_quantize_rows_i8(x.data_ptr(), DS_F32 if x.dtype is _F32 else DS_F16, ldx, out.data_ptr(), ldq, scale.data_ptr(), rows, Cch, st),
-          "ds_quantize_rows_i8")
-    return out, scale
+    return (_W8A8 or _w8a8()).quantize_rows_i8(x, out, scale, stream)
 
 
 def dequantize_rows_i8(q, scale, *, out=None, dtype=torch.float16, stream=None):
     """q * scale of each row, rounded once to `dtype` (fp16 / fp32)."""
-    rows, Cch, ldq = _rows_of(q, "dequantize_rows_i8(q)", _INT8)
-    if Cch < 1:
-        raise _lib.DsError("dequantize_rows_i8: rows without values")
-    _vector_of(scale, "dequantize_rows_i8(scale)", rows)
-    if out is None:
-        _rows_dtype("dequantize_rows_i8: dtype", dtype)
-        out, ldy = q.new_empty((rows, Cch), dtype=dtype), Cch
-    else:
-        ldy, dtype = _rows_of(out, "dequantize_rows_i8(out)", _ROWS, rows, Cch)[2], out.dtype
-    st = _stream_on(stream, q, scale, out)
-    check(_lib.load().ds_dequantize_rows_i8(q.data_ptr(), ldq, scale.data_ptr(), out.data_ptr(), DS_F32 if dtype is _F32 else DS_F16, ldy, rows, Cch, st),
-          "ds_dequantize_rows_i8")
-    return out
+    return (_W8A8 or _w8a8()).dequantize_rows_i8(q, scale, out, dtype, stream)
 
 
 def concat_channels(a, b, stream=None):
