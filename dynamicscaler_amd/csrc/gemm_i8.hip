@@ -28,20 +28,24 @@ struct I8Args {
 
 constexpr int BKB = 128;   // bytes (= values of k) of a K-step: 8 chunks of 16 bytes
 
-// 16 bytes of a row from byte `k` on, zeros behind the row's end: the last bytes are read as the 16 that end there, and shifted down
+// 16 bytes of a row from byte `k` on, zeros behind the row's end.  In two halves, so that several loads can be on their way: the last bytes are
+// read as the 16 that end with the row (rows of at least 16 bytes), and moved down when they have come.
 __device__ __forceinline__ u32x4 load_chunk(const int8_t* row, int k, int K) {
-    if (k + 16 <= K) return *reinterpret_cast<const u32x4_u*>(row + k);
+    if (K >= 16) return *reinterpret_cast<const u32x4_u*>(row + min(k, K - 16));
     u32x4 v = {0, 0, 0, 0};
-    if (k >= K) return v;
-    if (K >= 16) {
-        const u32x4 e = *reinterpret_cast<const u32x4_u*>(row + K - 16);
-        const unsigned long long lo = e[0] | (unsigned long long)e[1] << 32, hi = e[2] | (unsigned long long)e[3] << 32;
-        const int s = 8 * (k + 16 - K);          // 8 ... 120 bits
-        const unsigned long long l = s < 64 ? (lo >> s) | (hi << (64 - s)) : hi >> (s - 64), h = s < 64 ? hi >> s : 0;
-        return u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
-    }
     for (int j = 0; k + j < K; ++j) v[j >> 2] |= (unsigned)(uint8_t)row[k + j] << (8 * (j & 3));
     return v;
+}
+__device__ __forceinline__ u32x4 end_chunk(u32x4 v, int k, int K) {
+    const int bytes = k + 16 - K;
+    if (K < 16 || bytes <= 0) return v;
+    unsigned long long lo = v[0] | (unsigned long long)v[1] << 32, hi = v[2] | (unsigned long long)v[3] << 32;
+    if (bytes >= 8) { lo = hi; hi = 0; }
+    const int s = 8 * (bytes & 7);
+    lo = (lo >> s) | ((hi << 1) << (63 - s));
+    hi >>= s;
+    if (bytes >= 16) lo = hi = 0;
+    return u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
 }
 
 __device__ __forceinline__ float silu_f(float v) { return v / (1.0f + expf(-v)); }
@@ -158,15 +162,17 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
     }
     if (p.K % 64 != 0 && wave == waves - 1) {
         const int k = whole * 64 + 16 * l4;
-        i32x4 fw[NT];
+        u32x4 fw[NT], fa[MT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) fw[t] = (i32x4)load_chunk(w[t], k, p.K);
+        for (int t = 0; t < NT; ++t) fw[t] = load_chunk(w[t], k, p.K);
 #pragma unroll
-        for (int u = 0; u < MT; ++u) {
-            const i32x4 fa = (i32x4)load_chunk(a[u], k, p.K);
+        for (int u = 0; u < MT; ++u) fa[u] = load_chunk(a[u], k, p.K);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t], fa, acc[t][u], 0, 0, 0);
-        }
+        for (int t = 0; t < NT; ++t) fw[t] = end_chunk(fw[t], k, p.K);
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)fw[t], (i32x4)end_chunk(fa[u], k, p.K), acc[t][u], 0, 0, 0);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -204,24 +210,24 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, int8_t* dst, un
 }
 constexpr unsigned OOB = 0x80000000u;    // past every buffer (all are < 2 GiB)
 
-template <int BM, int BN, int WGM, int WGN> struct I8Tile {
+template <int BM, int BN, int WGM, int WGN, int NS> struct I8Tile {
     static constexpr int NT = 64 * WGM * WGN;
     static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
     static constexpr int LROWS = NT / 8, AR = BM / LROWS, BR = BN / LROWS;
-    static constexpr size_t STAGE = (size_t)(BM + BN) * BKB, LDS = 2 * STAGE;
+    static constexpr size_t STAGE = (size_t)(BM + BN) * BKB, LDS = NS * STAGE;
     static constexpr int PER_CU = (int)(163840 / LDS) * (NT / 64) > 16 ? 16 / (NT / 64) : (int)(163840 / LDS);
     static_assert(BM % (16 * WGM) == 0 && WN % 64 == 0 && BM % LROWS == 0 && BN % LROWS == 0 && LROWS % 32 == 0, "tile shape");
 };
 
-// Two LDS stages.  DMA (K % 16 == 0 and 16-byte aligned rows): both operands by LDS-DMA, the next K-step's pieces issued between the MFMAs of
-// this one.  Otherwise (any size, stride and alignment) through registers, loaded two K-steps ahead by unaligned 16-byte loads, rows past M / N
-// repeating the last one.  A stage holds BM rows of A, then BN rows of W, 128 bytes each, the 16-byte chunks XOR-swizzled through the SOURCE address so that a fragment
+// DMA (K % 16 == 0 and 16-byte aligned rows): both operands by LDS-DMA into NS stages, the pieces of K-step k + NS - 1 issued between the MFMAs
+// of k.  Otherwise (any size, stride and alignment) through registers into two stages, loaded D + 1 K-steps ahead by unaligned 16-byte loads,
+// rows past M / N repeating the last one.  A stage holds BM rows of A, then BN rows of W, 128 bytes each, the 16-byte chunks XOR-swizzled through the SOURCE address so that a fragment
 // read touches every bank once.  fp16 results: the wave's W rows are dealt to its MFMA tiles so that a lane ends up with 8 consecutive columns
-// (tile t, row i <-> column 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4) and a wave stores 64 contiguous bytes of 16 rows, as it does with the
-// natural order in fp32.
-template <int BM, int BN, int WGM, int WGN, bool DMA, bool OUT32, bool GEGLU>
-__global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * BN > 64 * 64 ? I8Tile<BM, BN, WGM, WGN>::PER_CU * I8Tile<BM, BN, WGM, WGN>::NT / 256 : 3)) gemm_i8_tile_kernel(I8Args p) {
-    using T = I8Tile<BM, BN, WGM, WGN>;
+// (tile t, row i <-> column 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4) as it does with 4 and the natural
+// order in fp32.
+template <int BM, int BN, int WGM, int WGN, int NS, bool DMA, bool STREAM, bool OUT32, bool GEGLU>
+__global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM * BN > 64 * 64 ? I8Tile<BM, BN, WGM, WGN, NS>::PER_CU * I8Tile<BM, BN, WGM, WGN, NS>::NT / 256 : 3)) gemm_i8_tile_kernel(I8Args p) {
+    using T = I8Tile<BM, BN, WGM, WGN, NS>;
     constexpr int TM = T::TM, TN = T::TN;
     extern __shared__ __attribute__((aligned(256))) int8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * B
     }
     const int last = p.K - (nk - 1) * BKB;      // bytes of the last K-step; chunks behind them bring zeros
     const unsigned cut_a = 16 * ca >= last ? OOB : 0u, cut_w = 16 * cw >= last ? OOB : 0u;
-    auto stage_row = [&](int j, int kt) { return smem + (kt & 1) * T::STAGE + (j < T::AR ? T::LROWS * j : BM + T::LROWS * (j - T::AR)) * BKB; };
+    auto stage_row = [&](int j, int kt) { return smem + (kt % NS) * T::STAGE + (j < T::AR ? T::LROWS * j : BM + T::LROWS * (j - T::AR)) * BKB; };
     auto piece = [&](int j, int kt) {
         const bool tail = kt == nk - 1;
         dma16(j < T::AR ? rsA : rsW, stage_row(j, kt) + 8 * wave * BKB, voff[j] | (tail ? (j < T::AR ? cut_a : cut_w) : 0u), (unsigned)kt * BKB);
@@ -279,6 +285,10 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * B
         }
     };
     auto store_regs = [&](int kt, int set) {
+        if (kt + 1 == nk && last != BKB) {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) reg[set][j] = end_chunk(reg[set][j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
+        }
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) *reinterpret_cast<u32x4*>(stage_row(j, kt) + srow * BKB + (tid & 7) * 16) = reg[set][j];
     };
@@ -287,29 +297,13 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * B
     for (int t = 0; t < TN; ++t)
 #pragma unroll
         for (int u = 0; u < TM; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
-    // every wave's pieces have landed and every wave is through with the other stage (lgkmcnt: its fragment reads, before they are overwritten)
-    auto sync = [&]() {
-        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    if constexpr (DMA) {
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) piece(j, 0);
-    } else if (nk > 0) {
-#pragma unroll
-        for (int d = 0; d < D; ++d)
-            if (d < nk) load_regs(d, d);
-        store_regs(0, 0);
-        if (D < nk) load_regs(D, 0);
-    }
-    // residual rows of a small wave tile: on their way while the product is formed
-    constexpr int G = OUT32 ? 1 : 2, CW = 4 * G;               // MFMA tiles and consecutive columns of a lane's group
-    constexpr int GROUPS = (GEGLU ? TN / 2 : TN) / G;
-    constexpr bool EARLY = !GEGLU && TM * TN <= 8;
+    constexpr int G = OUT32 ? 1 : 2, CW = 4 * G;               // a lane's consecutive columns on the way out, and their fours
+    // on the way out (GEGLU apart): lane -> row lane / LANES (+ 64 / LANES a turn) of a block of 16 RB rows, CW columns
+    constexpr int RB = TM < 2 || TM * TN > 16 || (size_t)T::NT / 2 * (T::WN + 4) * sizeof(float) > T::LDS ? 1 : 2, BLOCKS = TM / RB, LANES = T::WN / CW, TURNS = 16 * RB * LANES / 64;
     const int mw = m0 + wm * T::WM, nw = n0 + wn * T::WN;
-    u32x4 early[EARLY ? GROUPS : 1][EARLY ? TM : 1][G];
+    const int out_row = lane / LANES, out_col = nw + lane % LANES * CW;
+    constexpr int SETS = TM * TN > 16 && !OUT32 ? 1 : 2;       // (the 256 x 256 tile has no registers for a second set of fp16 results' residual)
+    u32x4 res[SETS][TURNS][G];
     auto load_residual = [&](int m, int col, u32x4* to) {
         const long at = (long)m * p.ldr + col;
 #pragma unroll
@@ -323,23 +317,46 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * B
             }
         }
     };
-    if (EARLY && p.residual) {
+    auto load_block = [&](int b) {
+        if (!GEGLU && p.residual && out_col + CW <= p.N) {
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            const int col = nw + 16 * g * G + CW * l4;
-#pragma unroll
-            for (int u = 0; u < TM; ++u)
-                if (col + CW <= p.N) load_residual(min(mw + 16 * u + l15, p.M - 1), col, early[g][u]);
+            for (int i = 0; i < TURNS; ++i) load_residual(min(mw + 16 * RB * b + out_row + 64 / LANES * i, p.M - 1), out_col, res[b % SETS][i]);
         }
+    };
+    constexpr bool EARLY = TM * TN <= 8;           // a small wave tile's residual is on its way while the product is formed
+    if (EARLY) load_block(0);
+    // the next K-step's pieces have landed for every wave (those of the NS - 2 steps behind it may be on their way) and every wave is through with
+    // the stage that is written next (lgkmcnt: its fragment reads)
+    auto sync = [&](bool all) {
+        if constexpr (!DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        else if (all || NS == 2) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PIECES * (NS - 2)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if constexpr (DMA) {
+#pragma unroll
+        for (int k = 0; k < NS - 1; ++k)
+            if (k < nk) {
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j) piece(j, k);
+            }
+    } else if (nk > 0) {
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (d < nk) load_regs(d, d);
+        store_regs(0, 0);
+        if (D < nk) load_regs(D, 0);
     }
-    sync();
-    auto kstep = [&](int kt, bool more, int set) {
+    sync(nk < NS - 1);
+    auto kstep = [&](int kt, int set) {
+        const bool more = DMA ? kt + NS - 1 < nk : kt + 1 < nk;
         if constexpr (!DMA) {        // K-step kt + 1 into the stage that every wave has left, the ones behind it on their way
             if (more) store_regs(kt + 1, set);
             if (kt + 1 + D < nk) load_regs(kt + 1 + D, set);
         }
-        const int8_t* sa = smem + (kt & 1) * T::STAGE + wm * T::WM * BKB;
-        const int8_t* sw = smem + (kt & 1) * T::STAGE + (BM + wn * T::WN) * BKB;
+        const int8_t* sa = smem + (kt % NS) * T::STAGE + wm * T::WM * BKB;
+        const int8_t* sw = smem + (kt % NS) * T::STAGE + (BM + wn * T::WN) * BKB;
         auto read_a = [&](int ks, int u) {
             const int row = u * 16 + l15;
             return *reinterpret_cast<const i32x4*>(sa + row * BKB + ((4 * ks + l4) ^ swz_a(row)) * 16);
@@ -375,28 +392,106 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * B
                 for (int j = 0; j < PIECES; ++j)
                     if (slot == ((j + 1) * SPAN) / PIECES - 1) {
                         __builtin_amdgcn_sched_barrier(0);
-                        if (DMA && more) piece(j, kt + 1);
+                        if (DMA && more) piece(j, kt + NS - 1);
                         __builtin_amdgcn_sched_barrier(0);
                     }
             }
         }
-        sync();
+        sync(!more);
     };
     for (int k0 = 0; k0 < nk; k0 += D)
 #pragma unroll
         for (int d = 0; d < D; ++d)
-            if (k0 + d < nk) kstep(k0 + d, k0 + d + 1 < nk, (d + 1) % D);
+            if (k0 + d < nk) kstep(k0 + d, (d + 1) % D);
 
-    // epilogue straight from the accumulators: 8 (fp16) or 4 (fp32) consecutive columns a lane
+    auto add_residual = [&](float* v, const u32x4* r) {
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+            if (p.epilogue & DS_EPI_RES_F32) v[j] += __uint_as_float(r[j / 4][j % 4]);
+            else v[j] += (float)__builtin_bit_cast(f16x2, (unsigned)r[j / 4][(j % 4) / 2])[j % 2];
+        }
+    };
+    // STREAM (results that L2 does not hold): past the cache, A rows and W panels stay (16384 x 2560 x 1280 in fp16: 85 -> 66 us)
+    auto store = [](auto v, auto* to) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+        else *to = v;
+    };
+    auto store_columns = [&](int m, int col, const float* v) {
+        const long at = (long)m * p.ldc + col;
+        if constexpr (OUT32) {
+            const f32x4 o = {v[0], v[1], v[2], v[3]};
+            store(o, reinterpret_cast<f32x4_u*>(reinterpret_cast<float*>(p.out) + at));
+        } else {
+            f16x8 h;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
+            store(h, reinterpret_cast<f16x8_u*>(reinterpret_cast<f16*>(p.out) + at));
+        }
+    };
     float sa[TM];
 #pragma unroll
     for (int u = 0; u < TM; ++u) sa[u] = p.a_scale[min(mw + 16 * u + l15, p.M - 1)];
+    // a large wave tile's fp16 results without a residual go straight out (40960 x 1280 x 1280: 92 us against 109)
+    const bool turned = !GEGLU && (OUT32 || TM * TN <= 16 || p.residual);
+    if (turned) {
+        // a wave turns its tile through a strip of LDS that is its own, 16 RB rows at a time: 256 (fp32) or 128 (fp16) contiguous bytes of a row
+        // go out together (655360 x 320 x 320 on fp32 rows: 495 -> 416 us); a block's residual is on its way while the one before it is stored
+        constexpr int LD = T::WN + 4;
+        static_assert((size_t)T::NT / 64 * 16 * RB * LD * sizeof(float) <= T::LDS, "strips");
+        float* strip = reinterpret_cast<float*>(smem) + wave * 16 * RB * LD;
+        if (!EARLY) load_block(0);
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            if (SETS == 2 && b + 1 < BLOCKS) load_block(b + 1);
+            if (SETS == 1 && b > 0) load_block(b);
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                f32x4 sw, bw;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int n = min(nw + (OUT32 ? 16 * t + 4 * l4 : 32 * (t >> 1) + 8 * l4 + 4 * (t & 1)) + j, p.N - 1);
+                    sw[j] = p.w_scale[n];
+                    bw[j] = p.bias ? p.bias[n] : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < RB; ++u) {
+                    f32x4 v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[j] = scaled(acc[t][RB * b + u][j], sa[RB * b + u], sw[j], bw[j]);
+                        if (p.epilogue & DS_EPI_SILU) v[j] = silu_f(v[j]);
+                    }
+                    *reinterpret_cast<f32x4*>(strip + (16 * u + l15) * LD + (OUT32 ? 16 * t + 4 * l4 : 32 * (t >> 1) + 8 * l4 + 4 * (t & 1))) = v;
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < TURNS; ++i) {
+                const int row = out_row + 64 / LANES * i, m = mw + 16 * RB * b + row;
+                float v[CW];
+#pragma unroll
+                for (int j = 0; j < CW; j += 4) *reinterpret_cast<f32x4*>(v + j) = *reinterpret_cast<const f32x4*>(strip + row * LD + lane % LANES * CW + j);
+                if (m >= p.M) continue;
+                if (out_col + CW <= p.N) {
+                    if (p.residual) add_residual(v, res[b % SETS][i]);
+                    store_columns(m, out_col, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < CW; ++j)
+                        if (out_col + j < p.N) store_at(p, m, out_col + j, v[j] + residual_at(p, m, out_col + j));
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        return;
+    }
+    // straight from the accumulators, 8 (fp16) or 4 (fp32) consecutive columns a lane; GEGLU: of every 64 columns 32 values, then their 32 gates
+    constexpr int GB = GEGLU ? 32 / (16 * G) : 1;              // a lane's value groups in a block of 64 columns
+    constexpr int GROUPS = (GEGLU ? TN / 2 : TN) / G;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-        // GEGLU: 64 columns = 32 values, 32 gates; value group g of 64-column block b, its gates 32 columns on
-        constexpr int GB = GEGLU ? 32 / (16 * G) : 1;          // groups of a 64-column block
-        const int t0 = GEGLU ? (g / GB) * 4 + (g % GB) * G : g * G;
-        const int nl = 16 * t0 + CW * l4, n = nw + nl;         // (tiles t0, t0 + 1 span 32 columns: lane l4 holds 8 l4 ... 8 l4 + 7 of them)
+        const int t0 = GEGLU ? g / GB * 4 + g % GB * G : g * G;        // first MFMA tile of the values; the gates' are two further
+        const int n = nw + 16 * t0 + CW * l4, col = GEGLU ? (nw + 64 * (g / GB)) / 2 + g % GB * 16 * G + CW * l4 : n;
         if (n >= p.N) continue;
         float sw[CW], bw[CW], sg[CW], bg[CW];
 #pragma unroll
@@ -409,8 +504,6 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * B
                 bg[j] = p.bias ? p.bias[c + 32] : 0.0f;
             }
         }
-        const int col = GEGLU ? (nw + 64 * (g / GB)) / 2 + (g % GB) * 16 * G + CW * l4 : n;
-        const int cols = GEGLU ? p.N / 2 : p.N;
 #pragma unroll
         for (int u = 0; u < TM; ++u) {
             const int m = mw + 16 * u + l15;
@@ -426,48 +519,26 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN>::NT), (DMA || BM * B
                     v[j] = silu_f(v[j]);
                 }
             }
-            if (col + CW <= cols) {
-                if (!GEGLU && p.residual) {
-                    u32x4 r[G];
-                    if constexpr (EARLY) {
-#pragma unroll
-                        for (int i = 0; i < G; ++i) r[i] = early[g][u][i];
-                    } else {
-                        load_residual(m, col, r);
-                    }
-#pragma unroll
-                    for (int j = 0; j < CW; ++j) {
-                        if (p.epilogue & DS_EPI_RES_F32) v[j] += __uint_as_float(r[j / 4][j % 4]);
-                        else v[j] += (float)__builtin_bit_cast(f16x2, (unsigned)r[j / 4][(j % 4) / 2])[j % 2];
-                    }
-                }
-                const long at = (long)m * p.ldc + col;
-                if constexpr (OUT32) {
-                    *reinterpret_cast<f32x4_u*>(reinterpret_cast<float*>(p.out) + at) = f32x4{v[0], v[1], v[2], v[3]};
-                } else {
-                    f16x8 h;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
-                    *reinterpret_cast<f16x8_u*>(reinterpret_cast<f16*>(p.out) + at) = h;
-                }
+            if (GEGLU || col + CW <= p.N) {
+                store_columns(m, col, v);
             } else {
 #pragma unroll
                 for (int j = 0; j < CW; ++j)
-                    if (col + j < cols) store_at(p, m, col + j, v[j] + residual_at(p, m, col + j));
+                    if (col + j < p.N) store_at(p, m, col + j, v[j]);
             }
         }
     }
 }
 
-template <int BM, int BN, int WGM, int WGN, bool DMA, bool OUT32, bool GEGLU>
+template <int BM, int BN, int WGM, int WGN, int NS, bool DMA, bool STREAM, bool OUT32, bool GEGLU>
 int launch_tile(I8Args p, hipStream_t st) {
-    using T = I8Tile<BM, BN, WGM, WGN>;
+    using T = I8Tile<BM, BN, WGM, WGN, NS>;
     p.tiles_m = ds_cdiv(p.M, BM);
     p.tiles_n = ds_cdiv(p.N, BN);
     const long tiles = (long)p.tiles_m * p.tiles_n;
     DS_CHECK_ARG(tiles * T::NT <= 0xffffffffL, "ds_gemm_i8: M %d x N %d has too many tiles for one launch", p.M, p.N);
     p.group_m = p.tiles_n > 8 ? 8 : 1;
-    auto kernel = gemm_i8_tile_kernel<BM, BN, WGM, WGN, DMA, OUT32, GEGLU>;
+    auto kernel = gemm_i8_tile_kernel<BM, BN, WGM, WGN, NS, DMA, STREAM, OUT32, GEGLU>;
     if (T::LDS > 65536) {
         hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::LDS);
         if (e != hipSuccess) { ds_set_error("ds_gemm_i8: %s", hipGetErrorString(e)); return DS_ELAUNCH; }
@@ -476,11 +547,60 @@ int launch_tile(I8Args p, hipStream_t st) {
     return DS_OK;
 }
 
-template <int BM, int BN, int WGM, int WGN, bool DMA>
+template <int BM, int BN, int WGM, int WGN, bool DMA, bool STREAM, int NS>
 int launch_tile(const I8Args& p, hipStream_t st) {
     const bool f32 = p.epilogue & DS_EPI_OUT_F32;
-    if (p.epilogue & DS_EPI_GEGLU) return f32 ? launch_tile<BM, BN, WGM, WGN, DMA, true, true>(p, st) : launch_tile<BM, BN, WGM, WGN, DMA, false, true>(p, st);
-    return f32 ? launch_tile<BM, BN, WGM, WGN, DMA, true, false>(p, st) : launch_tile<BM, BN, WGM, WGN, DMA, false, false>(p, st);
+    if (p.epilogue & DS_EPI_GEGLU)
+        return f32 ? launch_tile<BM, BN, WGM, WGN, NS, DMA, STREAM, true, true>(p, st) : launch_tile<BM, BN, WGM, WGN, NS, DMA, STREAM, false, true>(p, st);
+    return f32 ? launch_tile<BM, BN, WGM, WGN, NS, DMA, STREAM, true, false>(p, st) : launch_tile<BM, BN, WGM, WGN, NS, DMA, STREAM, false, false>(p, st);
+}
+
+template <int BM, int BN, int WGM, int WGN, bool DMA>
+int launch_large(const I8Args& p, bool stream_out, hipStream_t st) {
+    return stream_out ? launch_tile<BM, BN, WGM, WGN, DMA, true, 2>(p, st) : launch_tile<BM, BN, WGM, WGN, DMA, false, 2>(p, st);
+}
+
+// Which tile: the one whose estimate is the shortest.  Microseconds of a round (every workgroup that fits on the chip at once does one tile) =
+// start and end + (bytes per accumulator that go in and out with it) * b + K / 1024 * g, fitted to measurements of M = 300 ... 655360,
+// N = 320 ... 10240, K = 320 ... 8192, fp16 and fp32 results with and without a residual (within 20 %).  On either side of the choices: 8192^3 in
+// fp16 256 x 256 460 us, 128 x 128 582, 256 x 64 629, 128 x 64 688; 655360 x 320 x 320 on fp32 rows 553, 411, 387, 412; 2048 x 1280 x 1280
+// 64 x 64 9.9, 128 x 64 11.3, 256 x 256 20.5; 4096 x 1280 x 1280 64 x 64 16.8, 128 x 64 14.7, 128 x 128 16.4, 256 x 256 22.4.
+enum { TILE_256x256, TILE_128x128, TILE_256x64, TILE_128x64, TILE_64x64 };
+int choose_tile(const I8Args& p) {
+    struct Cost { int m, n, slots; double f, b, g; };
+    static const Cost cost[] = {{256, 256, 256, 5.2, 2.35, 11.6}, {128, 128, 512, 5.2, 0.72, 8.8}, {256, 64, 512, 5.0, 0.94, 9.6}, {128, 64, 768, 4.7, 0.68, 7.0}, {64, 64, 768, 4.0, 0.4, 4.3}};
+    double bytes = p.epilogue & DS_EPI_OUT_F32 ? 4 : 2;
+    if (p.epilogue & DS_EPI_GEGLU) bytes /= 2;
+    if (p.residual) bytes += p.epilogue & DS_EPI_RES_F32 ? 4 : 2;
+    int best = 0;
+    double least = 0;
+    for (int t = 0; t < 5; ++t) {
+        const Cost& c = cost[t];
+        const long tiles = (long)ds_cdiv(p.M, c.m) * ds_cdiv(p.N, c.n), rounds = (tiles + c.slots - 1) / c.slots;
+        const double part = (double)tiles / c.slots;          // several workgroups a CU: the next tiles begin before a round is over
+        const double us = (c.slots == 256 || rounds == 1 ? rounds : 0.5 * (rounds + part)) * (c.f + bytes * c.b + p.K / 1024.0 * c.g);
+        if (t == 0 || us < least) { best = t; least = us; }
+    }
+    const int forced = (int)DS_TUNE_INT("DS_I8_TILE", -1);     // (the "tune" build variant)
+    return forced >= 0 ? forced : best;
+}
+
+int launch_tiles(const I8Args& p, bool dma, hipStream_t st) {
+    // results that are more than L2 holds (32 MiB)
+    const bool stream_out = (long)p.M * p.N * (p.epilogue & DS_EPI_OUT_F32 ? 4 : 2) / (p.epilogue & DS_EPI_GEGLU ? 2 : 1) > (32 << 20);
+    if (!dma) {
+        // registers and unaligned loads: 64 x 64 up to one round of them (2057 x 997 x 1273: 19 us against 23), 128 x 128 behind (20057 x 1997 x 1273:
+        // 129 us against 186)
+        if ((long)ds_cdiv(p.M, 64) * ds_cdiv(p.N, 64) <= 768) return launch_tile<64, 64, 4, 1, false, false, 2>(p, st);
+        return launch_large<128, 128, 2, 2, false>(p, stream_out, st);
+    }
+    switch (choose_tile(p)) {
+        case TILE_256x256: return launch_large<256, 256, 2, 4, true>(p, stream_out, st);
+        case TILE_128x128: return launch_large<128, 128, 2, 2, true>(p, stream_out, st);
+        case TILE_256x64: return launch_large<256, 64, 8, 1, true>(p, stream_out, st);
+        case TILE_128x64: return launch_tile<128, 64, 4, 1, true, false, 2>(p, st);
+        default: return launch_tile<64, 64, 4, 1, true, false, 3>(p, st);
+    }
 }
 
 template <int MT>
@@ -528,17 +648,7 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
     else if (d.M <= 96) launch_few<6>(p, st);
     else if (d.M <= 128) launch_few<8>(p, st);
     else {
-        auto tiles = [&](int t) { return (long)ds_cdiv(d.M, t) * ds_cdiv(d.N, t); };
-        int rc;
-        if (dma) {
-            if (tiles(256) >= 256 && d.K >= 512) rc = launch_tile<256, 256, 2, 4, true>(p, st);
-            else if (tiles(128) >= 512 && d.K >= 512) rc = launch_tile<128, 128, 2, 2, true>(p, st);
-            else if ((long)ds_cdiv(d.M, 128) * ds_cdiv(d.N, 64) >= 256) rc = launch_tile<128, 64, 4, 1, true>(p, st);
-            else rc = launch_tile<64, 64, 4, 1, true>(p, st);
-        } else {
-            if (tiles(128) >= 512) rc = launch_tile<128, 128, 2, 2, false>(p, st);
-            else rc = launch_tile<64, 64, 4, 1, false>(p, st);
-        }
+        const int rc = launch_tiles(p, dma, st);
         if (rc != DS_OK) return rc;
     }
     DS_CHECK_LAUNCH("ds_gemm_i8");
