@@ -16,30 +16,23 @@ struct RowsArgs {
     long ldx, ldr, ldh, ldy;
     int C;
     float eps;
+    double inv_C;
 };
 
 template <typename T> __device__ __forceinline__ double as_f64(T v) { return (double)(float)v; }
 
-// rint(127 t / top), exactly: the quotient in 64 bits decides unless it is next to a half, where 254 |t| is compared with an odd multiple of
-// top (both exact for fp16 / fp32 t)
-__device__ __forceinline__ int quantum(double t, double top, double inv) {
-    const double v = fabs(t) * inv;
-    double q = rint(v);
-    if (fabs(fabs(v - q) - 0.5) < 1e-9) {
-        const double k = floor(v);                   // the half is k + 0.5
-        const double d = fma(-(2.0 * k + 1.0), top, 254.0 * fabs(t));
-        q = d > 0.0 ? k + 1.0 : d < 0.0 ? k : 2.0 * rint(0.5 * k + 0.25);
-    }
-    return t < 0.0 ? -(int)q : (int)q;
+// rint(127 t / top), exactly, from an estimate v of 127 |t| / top that is off by less than a quarter: 254 |t| against the odd multiple of top that
+// is the half above floor(v) (both exact for fp16 / fp32 t)
+__device__ __forceinline__ int quantum(double t, double top, double v) {
+    const double k = floor(v), d = fma(-fma(2.0, k, 1.0), top, 254.0 * fabs(t));
+    const int i = (int)k, q = i + (d > 0.0 || (d == 0.0 && (i & 1)) ? 1 : 0);
+    return t < 0.0 ? -q : q;
 }
 
-// The same from 32-bit forms: v = t inv carries at most five roundings of 2^-24 and |v| <= 127, so it is within 3.8e-5 of the quotient, and only
-// a fraction within 2^-14 of a half (one value in 8000) needs the 64-bit one.
-template <typename F> __device__ __forceinline__ int quantum_near(float v, F&& exactly) {
-    const float q = rintf(v);
-    int i = (int)q;
-    if (fabsf(v - q) > 0.5f - 0x1p-14f) i = exactly();
-    return i;
+// 1 / sqrt(s) for s > 0: the hardware's 2^-23 and one Newton step (2^-44); 0 for an infinite s
+__device__ __forceinline__ double inverse_root(double s) {
+    const double y = __builtin_amdgcn_rsq(s);
+    return s < __builtin_huge_val() ? y * fma(-0.5 * s * y, y, 1.5) : s != s ? s : 0.0;
 }
 
 // Sum / maximum over the T lanes of a team (a power of two, at most a wave), the same bits in every lane: two quad permutes, two mirrors,
@@ -206,12 +199,15 @@ __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p
                 top = fmax(top, s_top[turn][w]);
             }
         }
-        const double root = NORM ? 1.0 / sqrt(sum / C + (double)p.eps) : 1.0;
+        const double root = NORM ? inverse_root(sum * p.inv_C + (double)p.eps) : 1.0;
         const bool off = I8 && (!(sum < __builtin_huge_val()) || !(top < __builtin_huge_val()));
-        const double inv = I8 && top > 0.0 && !off ? 127.0 / top : 0.0;
-        const bool in32 = off || top == 0.0 || (top < 1e36 && top > 1e-30);       // t and 127 / top are ordinary fp32 numbers
-        const float inv32 = in32 ? (float)inv : 0.0f;
-        if (I8 && live && lane == 0) p.scale[row] = off ? __builtin_nanf("") : (float)(top * root / 127.0);
+        // 32-bit quotients v = t (127 / top): t carries two roundings of 2^-24, 127 / top two, v one -- within 3.8e-5 of the quotient, |v| <= 127 --
+        // decide all but the values within 2^-14 of a half (one in 8000); rows whose t or 127 / top are no ordinary fp32 numbers are done exactly
+        const bool in32 = off || top == 0.0 || (top < 1e36 && top > 1e-30);
+        const float inv32 = off || top == 0.0 || !in32 ? 0.0f : 127.0f / (float)top;
+        double inv = 0.0;
+        if (I8 && !in32) inv = 127.0 / top;
+        if (I8 && live && lane == 0) p.scale[row] = off ? __builtin_nanf("") : (float)(top * root * (1.0 / 127.0));
         Y* y = reinterpret_cast<Y*>(p.y) + rr * p.ldy;
         R* hs = reinterpret_cast<R*>(p.h) + rr * p.ldh;
 #pragma unroll
@@ -223,17 +219,30 @@ __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p
             const bool mine = live && chunk(v) < C;
             Chunk<Y> cy;
             cy.zero();
+            if constexpr (I8) {
+                int q[8];
+                bool near = !in32;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if constexpr (I8) {
+                for (int j = 0; j < 8; ++j) {
                     float t = cx[v].at(j);
                     if constexpr (RES) t += cr[v].at(j);
                     if constexpr (NORM) t *= g[v].at(j);
-                    if (in32) cy.put(j, quantum_near(off ? 0.0f : t * inv32, [&] { return quantum(t_of(v, j), top, inv); }));
-                    else cy.put(j, quantum(t_of(v, j), top, inv));
-                } else {
-                    cy.set(j, t_of(v, j) * root);
+                    const float w = off ? 0.0f : t * inv32, n = rintf(w);
+                    q[j] = (int)n;
+                    near |= fabsf(w - n) > 0.5f - 0x1p-14f;
                 }
+                if (near) {                  // once for the chunk, so that the way past it is short
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const double t = t_of(v, j);
+                        q[j] = quantum(t, top, in32 ? fabs((double)((float)t * inv32)) : fabs(t) * inv);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) cy.put(j, q[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) cy.set(j, t_of(v, j) * root);
             }
             if (mine) cy.store(y + at(v));
             if constexpr (RES) {
@@ -273,7 +282,7 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p) {
         sum += s_sum[w];
         top = fmax(top, s_top[w]);
     }
-    const double root = NORM ? 1.0 / sqrt(sum / p.C + (double)p.eps) : 1.0;
+    const double root = NORM ? inverse_root(sum * p.inv_C + (double)p.eps) : 1.0;
     if constexpr (sizeof(Y) == 1) {
         const bool bad = !(sum < __builtin_huge_val()) || !(top < __builtin_huge_val());
         const double inv = top > 0.0 && !bad ? 127.0 / top : 0.0;
@@ -281,7 +290,8 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p) {
         if (tid == 0) p.scale[row] = bad ? __builtin_nanf("") : (float)(top * root / 127.0);
         for (int c = tid; c < p.C; c += blockDim.x) {
             const double h = h_of(c);
-            q[c] = (int8_t)(inv > 0.0 ? quantum(NORM ? h * (double)p.g[c] : h, top, inv) : 0);
+            const double t = NORM ? h * (double)p.g[c] : h;
+            q[c] = (int8_t)(inv > 0.0 ? quantum(t, top, fabs(t) * inv) : 0);
             if constexpr (NORM) {
                 if (p.h) reinterpret_cast<R*>(p.h)[row * p.ldh + c] = (R)h;
             }
@@ -391,7 +401,7 @@ extern "C" int ds_rmsnorm_rows(const void* x, const void* residual, const float*
     DS_CHECK_ARG(ldx >= C && ldy >= C && (!residual || ldr >= C) && (!sum || lds >= C), "ds_rmsnorm_rows: a row stride is shorter than C %d", C);
     DS_CHECK_ARG(aligned(x, x_dtype) && aligned(residual, r_dtype) && aligned(sum, r_dtype) && aligned(y, y_dtype) && aligned(gamma, DS_F32) && aligned(scale, DS_F32),
                  "ds_rmsnorm_rows: a pointer is not aligned to its element");
-    const RowsArgs p{x, residual, gamma, sum, y, scale, ldx, ldr, lds, ldy, C, eps};
+    const RowsArgs p{x, residual, gamma, sum, y, scale, ldx, ldr, lds, ldy, C, eps, 1.0 / C};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const bool xf = x_dtype == DS_F32, rf = r_dtype == DS_F32;
     if (!residual) {
@@ -415,7 +425,7 @@ extern "C" int ds_quantize_rows_i8(const void* x, int x_dtype, int64_t ldx, int8
     DS_CHECK_ARG(x && q && scale, "ds_quantize_rows_i8: a pointer is NULL");
     DS_CHECK_ARG(ldx >= C && ldq >= C, "ds_quantize_rows_i8: a row stride is shorter than C %d", C);
     DS_CHECK_ARG(aligned(x, x_dtype) && aligned(scale, DS_F32), "ds_quantize_rows_i8: a pointer is not aligned to its element");
-    const RowsArgs p{x, nullptr, nullptr, nullptr, q, scale, ldx, 0, 0, ldq, C, 0.0f};
+    const RowsArgs p{x, nullptr, nullptr, nullptr, q, scale, ldx, 0, 0, ldq, C, 0.0f, 1.0 / C};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (x_dtype == DS_F32) launch_rows<float, f16, int8_t, false, false>(p, rows, st);
     else launch_rows<f16, f16, int8_t, false, false>(p, rows, st);
