@@ -15,6 +15,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 // the same 16 bytes at any address (global memory accepts them unaligned)
 typedef u32x4 __attribute__((aligned(1))) u32x4_u;
 typedef f16x8 __attribute__((aligned(2))) f16x8_u;
+typedef f16x4 __attribute__((aligned(2))) f16x4_u;
 typedef f32x4 __attribute__((aligned(4))) f32x4_u;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x4 __attribute__((aligned(4))) u32x4_4;
@@ -28,13 +29,43 @@ struct I8Args {
 
 constexpr int BKB = 128;   // bytes (= values of k) of a K-step: 8 chunks of 16 bytes
 
-// 16 bytes of a row from byte `k` on, zeros behind the row's end.  In two halves, so that several loads can be on their way: the last bytes are
-// read as the 16 that end with the row (rows of at least 16 bytes), and moved down when they have come.
-__device__ __forceinline__ u32x4 load_chunk(const int8_t* row, int k, int K) {
-    if (K >= 16) return *reinterpret_cast<const u32x4_u*>(row + min(k, K - 16));
-    u32x4 v = {0, 0, 0, 0};
-    for (int j = 0; k + j < K; ++j) v[j >> 2] |= (unsigned)(uint8_t)row[k + j] << (8 * (j & 3));
-    return v;
+// 16 bytes of a row from byte `k` on, zeros behind the row's end, in two halves so that several loads can be on their way: fetch() and, when they
+// have come, bytes().  The last bytes are fetched as the 16 that end with the row (rows of at least 16 bytes) and moved down afterwards.
+// ODD: addresses that are no multiple of 4 are read as the aligned dwords that hold the 16 bytes, five where they straddle -- each holds at
+// least one of them, so nothing outside the row's own dwords is touched -- and shifted into place: loads from odd addresses as such
+// take up to five times as long (16 x 4097 x 4095: 23 us; with K = 4092 6.8 us).
+template <bool ODD> struct Fetched {
+    u32x4 v;
+    unsigned e;
+    __device__ __forceinline__ void fetch(const int8_t* from) {
+        if constexpr (ODD) {
+            const unsigned s = (unsigned)(uintptr_t)from & 3;
+            const unsigned* at = reinterpret_cast<const unsigned*>(from - s);
+            v = *reinterpret_cast<const u32x4_4*>(at);
+            e = at[s ? 4 : 3];
+        } else {
+            v = *reinterpret_cast<const u32x4_u*>(from);
+        }
+    }
+    __device__ __forceinline__ u32x4 bytes(const int8_t* from) const {
+        if constexpr (!ODD) return v;
+        const unsigned s = (unsigned)(uintptr_t)from & 3;
+        return u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], s), __builtin_amdgcn_alignbyte(v[2], v[1], s), __builtin_amdgcn_alignbyte(v[3], v[2], s),
+                     __builtin_amdgcn_alignbyte(e, v[3], s)};
+    }
+};
+// the same where the row may end
+template <bool ODD> __device__ __forceinline__ void fetch_end(Fetched<ODD>& f, const int8_t* row, int k, int K) {
+    if (K >= 16) {
+        f.fetch(row + min(k, K - 16));
+        return;
+    }
+    f.v = u32x4{0, 0, 0, 0};
+    for (int j = 0; k + j < K; ++j) f.v[j >> 2] |= (unsigned)(uint8_t)row[k + j] << (8 * (j & 3));
+}
+__device__ __forceinline__ u32x4 end_chunk(u32x4 v, int k, int K);
+template <bool ODD> __device__ __forceinline__ u32x4 bytes_end(const Fetched<ODD>& f, const int8_t* row, int k, int K) {
+    return K >= 16 ? end_chunk(f.bytes(row + min(k, K - 16)), k, K) : f.v;
 }
 __device__ __forceinline__ u32x4 end_chunk(u32x4 v, int k, int K) {
     const int bytes = k + 16 - K;
@@ -92,10 +123,10 @@ __device__ __forceinline__ void store_at(const I8Args& p, int m, int n, float v)
 // waves of a workgroup: at most 16, and 64 KiB of partial sums
 template <int MT, bool GEGLU> struct Few {
     static constexpr int FIT = 64 / (MT * (GEGLU ? 2 : 1)), WAVES = FIT > 16 ? 16 : FIT;
-    static constexpr int U = MT == 1 ? (GEGLU ? 4 : 8) : MT <= 3 ? 4 : 2;      // blocks of 64 bytes whose loads a wave sends out together
+    static constexpr int U = MT == 1 ? (GEGLU ? 4 : 8) : MT == 2 && !GEGLU ? 4 : 2;      // blocks of 64 bytes whose loads a wave sends out together
 };
 
-template <int MT, bool GEGLU>
+template <int MT, bool GEGLU, bool ODD>
 __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kernel(I8Args p) {
     constexpr int NT = GEGLU ? 2 : 1, U = Few<MT, GEGLU>::U;
     extern __shared__ __attribute__((aligned(16))) i32x4 red[];      // [waves][NT][MT][64 lanes]
@@ -115,64 +146,76 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
         for (int u = 0; u < MT; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
     const int whole = p.K / 64, per = (whole + waves - 1) / waves;
     const int end = min(whole, (wave + 1) * per);
-    // what the epilogue needs is on its way while the product is formed
+    // What the epilogue needs is on its way while the product is formed -- as it lies in memory, since a conversion would wait for it -- and in
+    // whole fours where the 16 columns are all there: the instructions fetched are a large part of so short a kernel's time.
     const int col = GEGLU ? (blockIdx.x >> 1) * 32 + (blockIdx.x & 1) * 16 + 4 * l4 : n0 + 4 * l4, cols = GEGLU ? p.N / 2 : p.N;
-    float sw[NT][4], bw[NT][4], sa = 0.0f;
-    unsigned res[4];                     // the residual's bits as they came: a conversion here would wait for them
-    const bool res32 = p.epilogue & DS_EPI_RES_F32;
+    const bool full = GEGLU || n0 + 16 <= p.N, res32 = p.epilogue & DS_EPI_RES_F32;
+    f32x4 sw[NT], bw[NT];
+    float sa = 0.0f;
+    u32x4 res = {0, 0, 0, 0};
     auto row_data = [&](int u) {
         const int m = min(16 * u + l15, p.M - 1);
         sa = p.a_scale[m];
-        if (p.residual && res32) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const unsigned*>(p.residual)[(long)m * p.ldr + min(col + j, cols - 1)];
-        } else if (p.residual) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const uint16_t*>(p.residual)[(long)m * p.ldr + min(col + j, cols - 1)];
+        if (!p.residual) return;
+        const long at = (long)m * p.ldr + col;
+        if (full && res32) res = *reinterpret_cast<const u32x4_4*>(reinterpret_cast<const float*>(p.residual) + at);
+        else if (full) {
+            const u32x2_2 h = *reinterpret_cast<const u32x2_2*>(reinterpret_cast<const f16*>(p.residual) + at);
+            res[0] = h[0];
+            res[1] = h[1];
         }
     };
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+        const int n = n0 + 32 * t + 4 * l4;
+        bw[t] = f32x4{0, 0, 0, 0};
+        if (full) {
+            sw[t] = *reinterpret_cast<const f32x4_u*>(p.w_scale + n);
+            if (p.bias) bw[t] = *reinterpret_cast<const f32x4_u*>(p.bias + n);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = min(n0 + 32 * t + 4 * l4 + j, p.N - 1);
-            sw[t][j] = p.w_scale[n];
-            bw[t][j] = p.bias ? p.bias[n] : 0.0f;
+            for (int j = 0; j < 4; ++j) {
+                sw[t][j] = p.w_scale[min(n + j, p.N - 1)];
+                if (p.bias) bw[t][j] = p.bias[min(n + j, p.N - 1)];
+            }
         }
+    }
     if (wave < MT) row_data(wave);
     for (int b = wave * per; b < end; b += U) {
-        i32x4 fw[U][NT], fa[U][MT];
+        Fetched<ODD> fw[U][NT], fa[U][MT];
+        const int k = b * 64 + 16 * l4;
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (b + i < end) {
-                const int k = (b + i) * 64 + 16 * l4;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) fw[i][t] = (i32x4)*reinterpret_cast<const u32x4_u*>(w[t] + k);
+                for (int t = 0; t < NT; ++t) fw[i][t].fetch(w[t] + k + 64 * i);
 #pragma unroll
-                for (int u = 0; u < MT; ++u) fa[i][u] = (i32x4)*reinterpret_cast<const u32x4_u*>(a[u] + k);
+                for (int u = 0; u < MT; ++u) fa[i][u].fetch(a[u] + k + 64 * i);
             }
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (b + i < end) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int u = 0; u < MT; ++u) {
+                    const i32x4 av = (i32x4)fa[i][u].bytes(a[u]);
 #pragma unroll
-                    for (int u = 0; u < MT; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i][t], fa[i][u], acc[t][u], 0, 0, 0);
+                    for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)fw[i][t].bytes(w[t]), av, acc[t][u], 0, 0, 0);
+                }
             }
     }
     if (p.K % 64 != 0 && wave == waves - 1) {
         const int k = whole * 64 + 16 * l4;
-        u32x4 fw[NT], fa[MT];
+        Fetched<ODD> fw[NT], fa[MT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) fw[t] = load_chunk(w[t], k, p.K);
+        for (int t = 0; t < NT; ++t) fetch_end(fw[t], w[t], k, p.K);
 #pragma unroll
-        for (int u = 0; u < MT; ++u) fa[u] = load_chunk(a[u], k, p.K);
+        for (int u = 0; u < MT; ++u) fetch_end(fa[u], a[u], k, p.K);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) fw[t] = end_chunk(fw[t], k, p.K);
+        for (int u = 0; u < MT; ++u) {
+            const i32x4 av = (i32x4)bytes_end(fa[u], a[u], k, p.K);
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)fw[t], (i32x4)end_chunk(fa[u], k, p.K), acc[t][u], 0, 0, 0);
+            for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)bytes_end(fw[t], w[t], k, p.K), av, acc[t][u], 0, 0, 0);
+        }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -190,14 +233,28 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
         }
         const int m = 16 * u + l15;
         if (m >= p.M) continue;
+        float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (col + j >= cols) continue;
-            float v = scaled(sum[0][j], sa, sw[0][j], bw[0][j]);
-            if constexpr (GEGLU) v *= gelu_f(scaled(sum[NT - 1][j], sa, sw[NT - 1][j], bw[NT - 1][j]));
-            else if (p.epilogue & DS_EPI_SILU) v = silu_f(v);
-            if (p.residual) v += res32 ? __uint_as_float(res[j]) : (float)__builtin_bit_cast(f16, (uint16_t)res[j]);
-            store_at(p, m, col + j, v);
+            v[j] = scaled(sum[0][j], sa, sw[0][j], bw[0][j]);
+            if constexpr (GEGLU) v[j] *= gelu_f(scaled(sum[NT - 1][j], sa, sw[NT - 1][j], bw[NT - 1][j]));
+        }
+        if (!GEGLU && (p.epilogue & DS_EPI_SILU)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = silu_f(v[j]);
+        }
+        if (full) {
+            if (p.residual) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += res32 ? __uint_as_float(res[j]) : (float)__builtin_bit_cast(f16x2, (unsigned)res[j / 2])[j % 2];
+            }
+            const long at = (long)m * p.ldc + col;
+            if (p.epilogue & DS_EPI_OUT_F32) *reinterpret_cast<f32x4_u*>(reinterpret_cast<float*>(p.out) + at) = f32x4{v[0], v[1], v[2], v[3]};
+            else *reinterpret_cast<f16x4_u*>(reinterpret_cast<f16*>(p.out) + at) = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < cols) store_at(p, m, col + j, v[j] + residual_at(p, m, col + j));
         }
     }
 }
@@ -260,7 +317,7 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM
     unsigned voff[PIECES];
     const int8_t* src[PIECES];
     constexpr int D = !DMA && BM * BN <= 64 * 64 ? 2 : 1;       // K-steps held in registers on their way
-    u32x4 reg[D][PIECES];
+    Fetched<false> reg[D][PIECES];              // (reading aligned dwords gains nothing here: 129 x 4097 x 4095 35 us against 21)
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         const bool of_a = j < T::AR;
@@ -278,19 +335,19 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM
     auto load_regs = [&](int kt, int set) {
         if (kt + 1 < nk || last == BKB) {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) reg[set][j] = *reinterpret_cast<const u32x4_u*>(src[j] + kt * BKB + 16 * (j < T::AR ? ca : cw));
+            for (int j = 0; j < PIECES; ++j) reg[set][j].fetch(src[j] + kt * BKB + 16 * (j < T::AR ? ca : cw));
         } else {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) reg[set][j] = load_chunk(src[j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
+            for (int j = 0; j < PIECES; ++j) fetch_end(reg[set][j], src[j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
         }
     };
     auto store_regs = [&](int kt, int set) {
-        if (kt + 1 == nk && last != BKB) {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) reg[set][j] = end_chunk(reg[set][j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
+        for (int j = 0; j < PIECES; ++j) {
+            const bool whole = kt + 1 < nk || last == BKB;
+            const u32x4 v = whole ? reg[set][j].bytes(src[j]) : bytes_end(reg[set][j], src[j], kt * BKB + 16 * (j < T::AR ? ca : cw), p.K);
+            *reinterpret_cast<u32x4*>(stage_row(j, kt) + srow * BKB + (tid & 7) * 16) = v;
         }
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) *reinterpret_cast<u32x4*>(stage_row(j, kt) + srow * BKB + (tid & 7) * 16) = reg[set][j];
     };
     i32x4 acc[TN][TM];
 #pragma unroll
@@ -589,8 +646,7 @@ int launch_tiles(const I8Args& p, bool dma, hipStream_t st) {
     // results that are more than L2 holds (32 MiB)
     const bool stream_out = (long)p.M * p.N * (p.epilogue & DS_EPI_OUT_F32 ? 4 : 2) / (p.epilogue & DS_EPI_GEGLU ? 2 : 1) > (32 << 20);
     if (!dma) {
-        // registers and unaligned loads: 64 x 64 up to one round of them (2057 x 997 x 1273: 19 us against 23), 128 x 128 behind (20057 x 1997 x 1273:
-        // 129 us against 186)
+        // 64 x 64 up to one round of them (2057 x 997 x 1273: 19 us against 23), 128 x 128 behind (20057 x 1997 x 1273: 129 us against 186)
         if ((long)ds_cdiv(p.M, 64) * ds_cdiv(p.N, 64) <= 768) return launch_tile<64, 64, 4, 1, false, false, 2>(p, st);
         return launch_large<128, 128, 2, 2, false>(p, stream_out, st);
     }
@@ -603,16 +659,45 @@ int launch_tiles(const I8Args& p, bool dma, hipStream_t st) {
     }
 }
 
-template <int MT>
-void launch_few(const I8Args& p, hipStream_t st) {
+template <int MT, bool GEGLU>
+void launch_few(const I8Args& p, bool odd, hipStream_t st) {
+    using F = Few<MT, GEGLU>;
+    int waves = 1;                         // as many as let each have all its loads in flight at once
+    while (waves * 2 <= F::WAVES && waves * 64 * F::U < p.K) waves *= 2;
+    const size_t lds = (size_t)waves * MT * (GEGLU ? 2 : 1) * 1024;
+    const int grid = GEGLU ? p.N / 32 : ds_cdiv(p.N, 16);
+    if (odd) gemm_i8_few_kernel<MT, GEGLU, true><<<grid, waves * 64, lds, st>>>(p);
+    else gemm_i8_few_kernel<MT, GEGLU, false><<<grid, waves * 64, lds, st>>>(p);
+}
+
+// At most 64 rows: every workgroup of 16 columns reads all of A, so the few-rows kernel's time goes with (16 + M) N K at ~8.5 TB/s (a workgroup alone:
+// 34 GB/s; odd addresses and GEGLU's two weight rows 40 % of that); the 64 x 64 tiles take about as long for one row as for 64, by K,
+// while there are no more of them than CUs.  Microseconds of both, within 20 % at 1 ... 64 rows, N = 320 ... 40960, K = 320 ... 4096:
+// 16 x 1280 x 1280 3.3 against 6.0, 64 x 4096 x 4096 12.0 / 12.7, 32 x 10240 x 1280 8.6 / 7.1 (GEGLU 10.3 / 6.4), 48 x 40960 x 1280 26.9 / 12.5,
+// 32 x 4097 x 4095 18.2 / 21, 64 x 4097 x 4095 29.9 / 21.
+bool few_rows(const I8Args& p, bool dma, bool odd) {
+    if (p.M > 64) return false;
     const bool geglu = p.epilogue & DS_EPI_GEGLU;
-    // as many waves as let each have all its loads in flight at once
-    const int most = geglu ? Few<MT, true>::WAVES : Few<MT, false>::WAVES, batch = 64 * (geglu ? Few<MT, true>::U : Few<MT, false>::U);
-    int waves = 1;
-    while (waves * 2 <= most && waves * batch < p.K) waves *= 2;
-    const size_t lds = (size_t)waves * MT * (geglu ? 2 : 1) * 1024;
-    if (geglu) gemm_i8_few_kernel<MT, true><<<p.N / 32, waves * 64, lds, st>>>(p);
-    else gemm_i8_few_kernel<MT, false><<<ds_cdiv(p.N, 16), waves * 64, lds, st>>>(p);
+    const double k = p.K / 1024.0, rows = 16.0 * ds_cdiv(p.M, 16), groups = geglu ? p.N / 32 : ds_cdiv(p.N, 16);
+    const double mine = ((geglu ? 32 : 16) + rows) * k * 1024;          // bytes of a workgroup
+    const double all = groups * mine / 8.5e6 * (geglu ? 2.4 : 1.0), one = mine / 34e3, tiles = ds_cdiv(p.N, 64) / 256.0;
+    return 2.0 + (all > one ? all : one) * (odd ? 2.6 : 1.0) < (3.3 + (dma ? 2.3 : odd ? 4.4 : 3.5) * k) * (tiles > 1 ? 0.6 + 0.4 * tiles : 1.0);
+}
+
+int launch_i8(const I8Args& p, bool dma, bool odd, hipStream_t st) {
+    if (!few_rows(p, dma, odd)) return launch_tiles(p, dma, st);
+    const int tiles = ds_cdiv(p.M, 16);
+    if (p.epilogue & DS_EPI_GEGLU) {
+        if (tiles == 1) launch_few<1, true>(p, odd, st);
+        else if (tiles == 2) launch_few<2, true>(p, odd, st);
+        else launch_few<4, true>(p, odd, st);
+    } else {
+        if (tiles == 1) launch_few<1, false>(p, odd, st);
+        else if (tiles == 2) launch_few<2, false>(p, odd, st);
+        else if (tiles == 3) launch_few<3, false>(p, odd, st);
+        else launch_few<4, false>(p, odd, st);
+    }
+    return DS_OK;
 }
 
 }  // namespace
@@ -639,18 +724,11 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
                  "ds_gemm_i8: a pointer is not aligned to its element");
     I8Args p{A, W, a_scale, w_scale, bias, residual, out, d.lda, d.ldw, d.ldr, d.ldc, d.M, d.N, d.K, d.epilogue, 0, 0, 1};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const bool dma = d.K > 0 && (((uintptr_t)A | (uintptr_t)W) & 15) == 0 && ((d.lda | d.ldw | d.K) & 15) == 0 && 256 * d.lda < OOB && 256 * d.ldw < OOB;
-    if (d.M <= 16) launch_few<1>(p, st);
-    else if (d.M <= 32) launch_few<2>(p, st);
-    else if (d.M <= 48) launch_few<3>(p, st);
-    else if (d.M <= 64) launch_few<4>(p, st);
-    else if (d.M <= 80) launch_few<5>(p, st);
-    else if (d.M <= 96) launch_few<6>(p, st);
-    else if (d.M <= 128) launch_few<8>(p, st);
-    else {
-        const int rc = launch_tiles(p, dma, st);
-        if (rc != DS_OK) return rc;
-    }
+    const int64_t strides = d.lda | d.ldw;
+    const uintptr_t at = (uintptr_t)A | (uintptr_t)W;
+    const bool dma = d.K > 0 && ((at | strides | d.K) & 15) == 0 && 256 * d.lda < (int64_t)OOB && 256 * d.ldw < (int64_t)OOB;
+    const int rc = launch_i8(p, dma, ((at | strides) & 3) != 0, st);
+    if (rc != DS_OK) return rc;
     DS_CHECK_LAUNCH("ds_gemm_i8");
     return DS_OK;
 }

@@ -192,6 +192,50 @@ def test_product_rows_that_stand_for_zero_or_nan(m, n, k):
     assert not bool(got[keep_m, 3].isfinite()[0]) or bool((a[0].int() * w[3].int()).sum() == 0)
 
 
+def large_case(m, n, k, out_dtype, residual, act, seed=0):
+    """Operands on the device, and the definition in 64 bits there (elementary operations; the integer sums are exact in float64)."""
+    d = dev()
+    g = torch.Generator(device=d).manual_seed(seed)
+    a = torch.randint(-128, 128, (m, k), generator=g, device=d, dtype=torch.int16).to(torch.int8)
+    w = torch.randint(-128, 128, (n, k), generator=g, device=d, dtype=torch.int16).to(torch.int8)
+    cols = n // 2 if act == "geglu" else n
+    sa, sw = torch.rand(m, generator=g, device=d) * 0.02 + 1e-3, torch.rand(n, generator=g, device=d) * 0.02 / math.sqrt(k) + 1e-4
+    b = torch.randn(n, generator=g, device=d)
+    r = torch.randn((m, cols), generator=g, device=d).to(residual) if residual is not None else None
+    return (a, w, sa, sw, b, r), product_ref(a, w, sa, sw, b, r, act, out_dtype)
+
+
+# one size for each tile of the many-rows kernel (256 x 256, 128 x 128, 256 x 64, 128 x 64, 64 x 64; 128 x 128 and 64 x 64 through registers), with
+# rows and columns that end inside a tile, the last K-step cut, results below and above the size from which they pass the cache by
+@pytest.mark.parametrize("m,n,k", [(8200, 1296, 1040), (16500, 2576, 144), (8200, 2576, 1296), (20500, 656, 336), (40970, 320, 320), (4100, 1296, 1296), (1030, 656, 656),
+                                   (8211, 1297, 1043), (33000, 656, 333), (1030, 657, 655)])
+@pytest.mark.parametrize("out_dtype,residual,act", [(F16, None, "none"), (F16, F16, "none"), (F32, F32, "none"), (F32, None, "silu"), (F16, F32, "none"), (F16, None, "geglu"),
+                                                    (F32, None, "geglu")])
+def test_product_every_tile(m, n, k, out_dtype, residual, act):
+    from dynamicscaler_amd import ops
+    if act == "geglu":
+        n = n // 64 * 64
+    (a, w, sa, sw, b, r), (ref, before) = large_case(m, n, k, out_dtype, residual, act)
+    got = ops.gemm_i8(a, w, sa, sw, bias=b, residual=r, epilogue=EPI[act], out_dtype=out_dtype)
+    off = (got.double() - ref).abs()
+    tol = before + HALF[out_dtype] * (ref.abs() + before) + SUB[out_dtype]
+    assert got.dtype == out_dtype and float((off / tol).max()) <= 1.0
+    if residual == out_dtype:                    # the residual stream in place
+        assert ops.gemm_i8(a, w, sa, sw, bias=b, residual=r, epilogue=EPI[act], out=r) is r
+        assert torch.equal(r, got)
+
+
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 31, 33, 48, 49, 64, 65])
+@pytest.mark.parametrize("n,k", [(48, 64), (1280, 1280), (321, 1023), (130, 4095), (64, 13), (700, 66)])
+@pytest.mark.parametrize("act", ["none", "geglu"])
+def test_product_few_rows(m, n, k, act):
+    """Rows around the few-rows kernel's groups of 16, K split over its waves unevenly, odd addresses, columns that end inside a group."""
+    if act == "geglu":
+        n = max(64, n // 64 * 64)
+    c = product_case(m, n, k, m + n, residual=F16 if act == "none" else None, act=act)
+    close(run_product(c, act=act), *product_ref(*c, act), F16)
+
+
 def test_product_is_the_same_for_any_rows_of_the_launch():
     """Row m of a large launch equals the launch of row m alone, bit for bit (every tile shape adds the same exact sum)."""
     a, w, sa, sw, b, _ = product_case(700, 384, 640, 9)
@@ -416,6 +460,22 @@ def test_norm_in_place(m, n, dtype):
     y, _ = ops.rmsnorm(xd, g.to(d), residual=rd, sum_out=rd, out=xd)
     close(xd, t * root, 5 * H32 * (t * root).abs(), dtype)
     close(rd, h, H32 * h.abs(), dtype)
+
+
+@pytest.mark.parametrize("m,n", [(5000, 320), (2051, 1283), (1100, 5120), (1027, 9000), (300, 16384)])
+def test_many_rows(m, n):
+    """More rows than a launch has teams: a team's later rows, gamma kept between them; every row against the definition."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    x, g, r = row_inputs(m, n, 3, F16), 1.0 + 0.2 * normal((n,), n), normal((m, n), 4, F32)
+    h, t, root = rows_ref(x, r, g, 1e-6, True)
+    q, scale, back = ops.rmsnorm_i8(x.to(d), g.to(d), residual=r.to(d))
+    check_rows_i8(q, scale, t, root)
+    close(back, h, H32 * h.abs(), F32)
+    q, scale = ops.quantize_rows_i8(x.to(d))
+    check_rows_i8(q, scale, x.double(), torch.ones(m, 1, dtype=torch.float64))
+    v = q.cpu().double() * scale.cpu().double()[:, None]
+    close(ops.dequantize_rows_i8(q, scale), v, H32 * v.abs(), F16)
 
 
 def test_rows_of_nothing():
