@@ -116,7 +116,8 @@ SIGNATURES = {
     "ds_clip_preprocess": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "ds_patchify": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "ds_cast_to_f16": (_i, [_vp, _i, _vp, _sz, _vp]),
-    "ds_gemm_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _pp(GemmI8Desc), _vp]),
+    "ds_gemm_i8_workspace_bytes": (_sz, [_vp, _vp, _pp(GemmI8Desc)]),
+    "ds_gemm_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _pp(GemmI8Desc), _vp, _sz, _vp]),
     "ds_rmsnorm_rows": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _pp(RmsnormDesc), _vp]),
     "ds_quantize_rows_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i, _i, _vp]),
     "ds_dequantize_rows_i8": (_i, [_vp, _i64, _vp, _vp, _i, _i64, _i, _i, _vp]),
@@ -202,8 +203,8 @@ def load_w8a8():
             from . import _w8a8 as front
         except ImportError as e:
             raise HipLibraryMissing(f"cannot load {os.path.join(HERE, '_w8a8.so')}: build it with `python -m dynamicscaler_amd.build` ({e})") from e
-        front.bind(DsError, *(C.cast(f, C.c_void_p).value for f in (lib.ds_gemm_i8, lib.ds_rmsnorm_rows, lib.ds_quantize_rows_i8, lib.ds_dequantize_rows_i8,
-                                                                  lib.ds_last_error)))
+        front.bind(DsError, *(C.cast(f, C.c_void_p).value for f in (lib.ds_gemm_i8_workspace_bytes, lib.ds_gemm_i8, lib.ds_rmsnorm_rows,
+                                                                  lib.ds_quantize_rows_i8, lib.ds_dequantize_rows_i8, lib.ds_last_error)))
         _w8a8 = front
     return _w8a8
 

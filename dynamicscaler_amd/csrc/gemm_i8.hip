@@ -488,8 +488,9 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM
     float sa[TM];
 #pragma unroll
     for (int u = 0; u < TM; ++u) sa[u] = p.a_scale[min(mw + 16 * u + l15, p.M - 1)];
-    // a large wave tile's fp16 results without a residual go straight out (40960 x 1280 x 1280: 92 us against 109)
-    const bool turned = !GEGLU && (OUT32 || TM * TN <= 16 || p.residual);
+    // a large wave tile's fp16 results without a residual go straight out (40960 x 1280 x 1280: 85 us against 102) where its 64-byte pieces are whole
+    // ones (100001 x 2008 x 1008: 392 us straight)
+    const bool turned = !GEGLU && (OUT32 || TM * TN <= 16 || p.residual || (p.ldc & 31) || ((uintptr_t)p.out & 63));
     if (turned) {
         // a wave turns its tile through a strip of LDS that is its own, 16 RB rows at a time: 256 (fp32) or 128 (fp16) contiguous bytes of a row
         // go out together (655360 x 320 x 320 on fp32 rows: 495 -> 416 us); a block's residual is on its way while the one before it is stored
@@ -583,6 +584,25 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM
                 for (int j = 0; j < CW; ++j)
                     if (col + j < p.N) store_at(p, m, col + j, v[j]);
             }
+        }
+    }
+}
+
+// Rows of K bytes at any address into rows of K rounded up to 16, zeros behind, which is what LDS-DMA takes: both operands in one launch, A's rows
+// first.  Teams of 1 << shift lanes a row, 16 bytes a lane and turn.
+struct AlignArgs { const int8_t* A; const int8_t* W; int8_t* to_a; int8_t* to_w; long lda, ldw; int M, N, K, stride, shift; };
+__global__ void __launch_bounds__(256) align_rows_kernel(AlignArgs p) {
+    const int team = 256 >> p.shift, lane = threadIdx.x & ((1 << p.shift) - 1);
+    const long rows_a = p.to_a ? p.M : 0, rows = rows_a + (p.to_w ? p.N : 0);
+    for (long row = (long)blockIdx.x * team + (threadIdx.x >> p.shift); row < rows; row += (long)gridDim.x * team) {
+        const bool of_a = row < rows_a;
+        const long at = of_a ? row : row - rows_a;
+        const int8_t* src = of_a ? p.A + at * p.lda : p.W + at * p.ldw;
+        int8_t* dst = (of_a ? p.to_a : p.to_w) + at * p.stride;
+        for (int k = 16 * lane; k < p.stride; k += 16 << p.shift) {
+            Fetched<true> f;
+            fetch_end(f, src, k, p.K);
+            *reinterpret_cast<u32x4*>(dst + k) = bytes_end(f, src, k, p.K);
         }
     }
 }
@@ -684,6 +704,38 @@ bool few_rows(const I8Args& p, bool dma, bool odd) {
     return 2.0 + (all > one ? all : one) * (odd ? 2.6 : 1.0) < (3.3 + (dma ? 2.3 : odd ? 4.4 : 3.5) * k) * (tiles > 1 ? 0.6 + 0.4 * tiles : 1.0);
 }
 
+struct Aligned { bool a, w; size_t bytes_a, bytes_w; int stride; };      // which operands to lay out anew, and where that ends
+bool dma_rows(const int8_t* p, int64_t ld, int K) { return ((uintptr_t)p & 15) == 0 && (ld & 15) == 0 && (K & 15) == 0 && 256 * ld < (int64_t)OOB; }
+
+// Operands that LDS-DMA does not take are worth a copy for it where the copy (a launch of ~2 us, in and out at ~4.5 TB/s) costs less than the
+// unaligned loads of the product, 0.75 us a K-step for every round of 768 64 x 64 tiles.  With and without: 2057 x 997 x 1273 17.7 and 19.6 us,
+// 20057 x 1997 x 1273 97 and 126, 100001 x 2001 x 1001 337 and 488, 1000 x 4097 x 4095 42 and 63; not worth it: 1000 x 997 x 1273 12.6 and
+// 10.4, 129 x 4097 x 4095 24.8 and 21.9.
+Aligned aligned_copies(const ds_gemm_i8_desc& d, const int8_t* A, const int8_t* W) {
+    Aligned c{false, false, 0, 0, (d.K + 15) / 16 * 16};
+    if (d.M <= 64 || d.N <= 0 || d.K < 16) return c;
+    const bool a = !dma_rows(A, d.lda, d.K), w = !dma_rows(W, d.ldw, d.K);
+    const double rounds = (double)ds_cdiv(d.M, 64) * ds_cdiv(d.N, 64) / 768;
+    const double moved = 2.0 * d.K * ((a ? d.M : 0.0) + (w ? d.N : 0.0));
+    if (!(a || w) || 2.2 + moved / 4.5e6 > 0.75 * d.K / BKB * rounds) return c;
+    c.a = a;
+    c.w = w;
+    c.bytes_a = a ? (size_t)d.M * c.stride : 0;                          // (rows of whole 16s: W's copy begins at a multiple of 16)
+    c.bytes_w = w ? (size_t)d.N * c.stride : 0;
+    return c;
+}
+
+void align_operands(I8Args& p, const Aligned& c, void* workspace, hipStream_t st) {
+    AlignArgs q{p.A, p.W, c.a ? static_cast<int8_t*>(workspace) : nullptr, c.w ? static_cast<int8_t*>(workspace) + c.bytes_a : nullptr, p.lda, p.ldw, p.M, p.N, p.K, c.stride, 3};
+    while (q.shift < 8 && (16 << q.shift) < c.stride) ++q.shift;
+    const long rows = (c.a ? p.M : 0L) + (c.w ? p.N : 0L);
+    const long groups = (rows + (256 >> q.shift) - 1) / (256 >> q.shift);
+    align_rows_kernel<<<(int)(groups < (1 << 20) ? groups : 1 << 20), 256, 0, st>>>(q);
+    if (c.a) { p.A = q.to_a; p.lda = c.stride; }
+    if (c.w) { p.W = q.to_w; p.ldw = c.stride; }
+    p.K = c.stride;                                                       // one side of every product behind K is a zero
+}
+
 int launch_i8(const I8Args& p, bool dma, bool odd, hipStream_t st) {
     if (!few_rows(p, dma, odd)) return launch_tiles(p, dma, st);
     const int tiles = ds_cdiv(p.M, 16);
@@ -702,8 +754,14 @@ int launch_i8(const I8Args& p, bool dma, bool odd, hipStream_t st) {
 
 }  // namespace
 
+extern "C" size_t ds_gemm_i8_workspace_bytes(const int8_t* A, const int8_t* W, const ds_gemm_i8_desc* desc) {
+    if (!desc) return 0;
+    const Aligned c = aligned_copies(*desc, A, W);
+    return c.bytes_a + c.bytes_w;
+}
+
 extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale, const float* w_scale, const float* bias, const void* residual,
-                          void* out, const ds_gemm_i8_desc* desc, void* stream) {
+                          void* out, const ds_gemm_i8_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
     DS_CHECK_ARG(desc, "ds_gemm_i8: desc is NULL");
     const ds_gemm_i8_desc d = *desc;
     DS_CHECK_ARG(d.M >= 0 && d.N >= 0 && d.K >= 0, "ds_gemm_i8: negative size (M %d, N %d, K %d)", d.M, d.N, d.K);
@@ -724,10 +782,14 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
                  "ds_gemm_i8: a pointer is not aligned to its element");
     I8Args p{A, W, a_scale, w_scale, bias, residual, out, d.lda, d.ldw, d.ldr, d.ldc, d.M, d.N, d.K, d.epilogue, 0, 0, 1};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const int64_t strides = d.lda | d.ldw;
-    const uintptr_t at = (uintptr_t)A | (uintptr_t)W;
-    const bool dma = d.K > 0 && ((at | strides | d.K) & 15) == 0 && 256 * d.lda < (int64_t)OOB && 256 * d.ldw < (int64_t)OOB;
-    const int rc = launch_i8(p, dma, ((at | strides) & 3) != 0, st);
+    const Aligned copies = aligned_copies(d, A, W);
+    if (workspace && copies.bytes_a + copies.bytes_w) {
+        DS_CHECK_ARG(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= copies.bytes_a + copies.bytes_w,
+                     "ds_gemm_i8: workspace of %zu bytes: %zu at a multiple of 16 are needed", workspace_bytes, copies.bytes_a + copies.bytes_w);
+        align_operands(p, copies, workspace, st);
+    }
+    const bool dma = p.K > 0 && dma_rows(p.A, p.lda, p.K) && dma_rows(p.W, p.ldw, p.K);
+    const int rc = launch_i8(p, dma, (((uintptr_t)p.A | (uintptr_t)p.W | p.lda | p.ldw) & 3) != 0, st);
     if (rc != DS_OK) return rc;
     DS_CHECK_LAUNCH("ds_gemm_i8");
     return DS_OK;

@@ -255,53 +255,52 @@ __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p
     }
 }
 
-// Longer rows, and rows of less than 8 values: one workgroup per row, the row read for the sums and again for the result.
+// Longer rows, and rows of less than 8 values: one workgroup per row and turn, the row read for the sums and again for the result.
 template <typename X, typename R, typename Y, bool NORM>
-__global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p) {
-    __shared__ double s_sum[16];
-    __shared__ double s_top[16];
-    const long row = blockIdx.x;
+__global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p, int rows) {
+    __shared__ double s_sum[16], s_top[16];
     const int tid = threadIdx.x;
-    const X* x = reinterpret_cast<const X*>(p.x) + row * p.ldx;
-    const R* r = p.r ? reinterpret_cast<const R*>(p.r) + row * p.ldr : nullptr;
-    auto h_of = [&](int c) { return r ? as_f64(x[c]) + as_f64(r[c]) : as_f64(x[c]); };
-    double sum = 0.0;
-    double top = 0.0;
-    for (int c = tid; c < p.C; c += blockDim.x) {
-        const double h = h_of(c);
-        sum += h * h;
-        const double t = fabs(NORM ? h * (double)p.g[c] : h);
-        top = fmax(top, t < __builtin_huge_val() ? t : __builtin_huge_val());        // an infinity stands for NaN too
-    }
-    sum = team_sum<64>(sum);
-    top = team_max<64>(top);
-    if ((tid & 63) == 0) { s_sum[tid >> 6] = sum; s_top[tid >> 6] = top; }
-    __syncthreads();
-    sum = 0.0;
-    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
-        sum += s_sum[w];
-        top = fmax(top, s_top[w]);
-    }
-    const double root = NORM ? inverse_root(sum * p.inv_C + (double)p.eps) : 1.0;
-    if constexpr (sizeof(Y) == 1) {
-        const bool bad = !(sum < __builtin_huge_val()) || !(top < __builtin_huge_val());
-        const double inv = top > 0.0 && !bad ? 127.0 / top : 0.0;
-        int8_t* q = reinterpret_cast<int8_t*>(p.y) + row * p.ldy;
-        if (tid == 0) p.scale[row] = bad ? __builtin_nanf("") : (float)(top * root / 127.0);
+    for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const X* x = reinterpret_cast<const X*>(p.x) + row * p.ldx;
+        const R* r = p.r ? reinterpret_cast<const R*>(p.r) + row * p.ldr : nullptr;
+        auto h_of = [&](int c) { return r ? as_f64(x[c]) + as_f64(r[c]) : as_f64(x[c]); };
+        double sum = 0.0, top = 0.0;
         for (int c = tid; c < p.C; c += blockDim.x) {
             const double h = h_of(c);
-            const double t = NORM ? h * (double)p.g[c] : h;
-            q[c] = (int8_t)(inv > 0.0 ? quantum(t, top, fabs(t) * inv) : 0);
-            if constexpr (NORM) {
+            sum += h * h;
+            const double t = fabs(NORM ? h * (double)p.g[c] : h);
+            top = fmax(top, t < __builtin_huge_val() ? t : __builtin_huge_val());        // an infinity stands for NaN too
+        }
+        sum = team_sum<64>(sum);
+        top = team_max<64>(top);
+        __syncthreads();                     // the row before has been read
+        if ((tid & 63) == 0) { s_sum[tid >> 6] = sum; s_top[tid >> 6] = top; }
+        __syncthreads();
+        sum = 0.0;
+        for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+            sum += s_sum[w];
+            top = fmax(top, s_top[w]);
+        }
+        const double root = NORM ? inverse_root(sum * p.inv_C + (double)p.eps) : 1.0;
+        if constexpr (sizeof(Y) == 1) {
+            const bool bad = !(sum < __builtin_huge_val()) || !(top < __builtin_huge_val());
+            const double inv = top > 0.0 && !bad ? 127.0 / top : 0.0;
+            int8_t* q = reinterpret_cast<int8_t*>(p.y) + row * p.ldy;
+            if (tid == 0) p.scale[row] = bad ? __builtin_nanf("") : (float)(top * root * (1.0 / 127.0));
+            for (int c = tid; c < p.C; c += blockDim.x) {
+                const double h = h_of(c), t = NORM ? h * (double)p.g[c] : h;
+                q[c] = (int8_t)(inv > 0.0 ? quantum(t, top, fabs(t) * inv) : 0);
+                if constexpr (NORM) {
+                    if (p.h) reinterpret_cast<R*>(p.h)[row * p.ldh + c] = (R)h;
+                }
+            }
+        } else {
+            Y* y = reinterpret_cast<Y*>(p.y) + row * p.ldy;
+            for (int c = tid; c < p.C; c += blockDim.x) {
+                const double h = h_of(c);
+                y[c] = (Y)(float)(h * root * (double)p.g[c]);
                 if (p.h) reinterpret_cast<R*>(p.h)[row * p.ldh + c] = (R)h;
             }
-        }
-    } else {
-        Y* y = reinterpret_cast<Y*>(p.y) + row * p.ldy;
-        for (int c = tid; c < p.C; c += blockDim.x) {
-            const double h = h_of(c);
-            y[c] = (Y)(float)(h * root * (double)p.g[c]);
-            if (p.h) reinterpret_cast<R*>(p.h)[row * p.ldh + c] = (R)h;
         }
     }
 }
@@ -331,10 +330,11 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__
 
 // ... and value by value: rows of less than 8 values, or of more chunks than `magic` takes
 template <typename Y>
-__global__ void __launch_bounds__(256) dequant_any_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int C) {
-    const long row = blockIdx.x;
-    const float s = scale[row];
-    for (int c = threadIdx.x; c < C; c += 256) y[row * ldy + c] = (Y)((float)q[row * ldq + c] * s);
+__global__ void __launch_bounds__(256) dequant_any_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C) {
+    for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float s = scale[row];
+        for (int c = threadIdx.x; c < C; c += blockDim.x) y[row * ldy + c] = (Y)((float)q[row * ldq + c] * s);
+    }
 }
 
 template <typename Y>
@@ -343,7 +343,7 @@ void launch_dequant(const int8_t* q, long ldq, const float* scale, Y* y, long ld
     const long chunks = (long)per_row * rows;
     const int span = chunks >= 1024 * 1024 ? 1024 : 256;        // four chunks a lane once they fill the chip
     if (C < 8 || per_row + span >= 65536 || ds_cdiv(chunks, span) > 0xffffff) {
-        dequant_any_kernel<Y><<<rows, 256, 0, st>>>(q, ldq, scale, y, ldy, C);
+        dequant_any_kernel<Y><<<rows < (1 << 20) ? rows : 1 << 20, C < 64 ? 64 : 256, 0, st>>>(q, ldq, scale, y, ldy, rows, C);
         return;
     }
     const unsigned long long magic = ((1ull << 40) + per_row - 1) / per_row;
@@ -358,8 +358,9 @@ void launch_rows(const RowsArgs& p, int rows, hipStream_t st) {
     // the smallest team whose four chunks a lane hold the row; a norm's teams walk several rows, with gamma in registers, once the chip is
     // full (16 waves a CU)
     constexpr int V = 4;
-    auto grid = [&](int teams) { const int n = ds_cdiv(rows, teams); return NORM && n > 256 * 4 ? 256 * 4 : n; };
-    if (p.C < 8) rows_long_kernel<X, R, Y, NORM><<<rows, 64, 0, st>>>(p);
+    constexpr int MOST = 1 << 20;        // workgroups of a launch: every kernel walks what is left
+    auto grid = [&](int teams) { const int n = ds_cdiv(rows, teams), most = NORM ? 256 * 4 : MOST; return n < most ? n : most; };
+    if (p.C < 8) rows_long_kernel<X, R, Y, NORM><<<rows < MOST ? rows : MOST, 64, 0, st>>>(p, rows);
     else if (p.C <= 8 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 8, V><<<grid(32), 256, 0, st>>>(p, rows);
     else if (p.C <= 16 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 16, V><<<grid(16), 256, 0, st>>>(p, rows);
     else if (p.C <= 32 * 8 * V) rows_team_kernel<X, R, Y, NORM, RES, 32, V><<<grid(8), 256, 0, st>>>(p, rows);
@@ -373,7 +374,7 @@ void launch_rows(const RowsArgs& p, int rows, hipStream_t st) {
                 return;
             }
         }
-        rows_long_kernel<X, R, Y, NORM><<<rows, 1024, 0, st>>>(p);
+        rows_long_kernel<X, R, Y, NORM><<<rows < MOST ? rows : MOST, 1024, 0, st>>>(p, rows);
     }
 }
 

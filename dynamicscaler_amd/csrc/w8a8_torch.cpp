@@ -14,6 +14,7 @@
 
 namespace {
 
+decltype(&ds_gemm_i8_workspace_bytes) c_gemm_workspace;
 decltype(&ds_gemm_i8) c_gemm;
 decltype(&ds_rmsnorm_rows) c_rmsnorm;
 decltype(&ds_quantize_rows_i8) c_quantize;
@@ -192,8 +193,13 @@ PyObject* gemm_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
             out = call.empty({a.m, cols}, type);
             d.ldc = cols;
         }
-        done(c_gemm(static_cast<const int8_t*>(A.const_data_ptr()), static_cast<const int8_t*>(W.const_data_ptr()), static_cast<const float*>(sa.const_data_ptr()),
-                    static_cast<const float*>(sw.const_data_ptr()), bias, residual, out.data_ptr(), &d, st), "ds_gemm_i8");
+        const int8_t *pa = static_cast<const int8_t*>(A.const_data_ptr()), *pw = static_cast<const int8_t*>(W.const_data_ptr());
+        // the workspace goes back to the allocator with the call, so it is one of the current stream's: a call that names another does without
+        at::Tensor room;
+        const size_t bytes = arg[9] == Py_None ? c_gemm_workspace(pa, pw, &d) : 0;
+        if (bytes) room = call.empty({(int64_t)bytes}, at::kChar);
+        done(c_gemm(pa, pw, static_cast<const float*>(sa.const_data_ptr()), static_cast<const float*>(sw.const_data_ptr()), bias, residual, out.data_ptr(), &d,
+                    bytes ? room.data_ptr() : nullptr, bytes, st), "ds_gemm_i8");
         return handed(arg[6], out);
     });
 }
@@ -311,16 +317,17 @@ PyObject* dequantize_rows_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) 
     });
 }
 
-// the exception class and the entries' addresses (gemm, rmsnorm, quantize, dequantize, last_error)
+// the exception class and the entries' addresses (gemm's workspace, gemm, rmsnorm, quantize, dequantize, last_error)
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject* cls;
-    unsigned long long f[5];
-    if (!PyArg_ParseTuple(args, "OKKKKK", &cls, &f[0], &f[1], &f[2], &f[3], &f[4])) return nullptr;
-    c_gemm = reinterpret_cast<decltype(c_gemm)>(f[0]);
-    c_rmsnorm = reinterpret_cast<decltype(c_rmsnorm)>(f[1]);
-    c_quantize = reinterpret_cast<decltype(c_quantize)>(f[2]);
-    c_dequantize = reinterpret_cast<decltype(c_dequantize)>(f[3]);
-    c_last_error = reinterpret_cast<decltype(c_last_error)>(f[4]);
+    unsigned long long f[6];
+    if (!PyArg_ParseTuple(args, "OKKKKKK", &cls, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5])) return nullptr;
+    c_gemm_workspace = reinterpret_cast<decltype(c_gemm_workspace)>(f[0]);
+    c_gemm = reinterpret_cast<decltype(c_gemm)>(f[1]);
+    c_rmsnorm = reinterpret_cast<decltype(c_rmsnorm)>(f[2]);
+    c_quantize = reinterpret_cast<decltype(c_quantize)>(f[3]);
+    c_dequantize = reinterpret_cast<decltype(c_dequantize)>(f[4]);
+    c_last_error = reinterpret_cast<decltype(c_last_error)>(f[5]);
     Py_INCREF(cls);
     Py_XDECREF(ds_error);
     ds_error = cls;

@@ -355,9 +355,12 @@ typedef struct ds_gemm_i8_desc {
  * A int8 [M][lda], W int8 [N][ldw], a_scale [M], w_scale [N], bias [N] or NULL (fp32); residual fp16 (fp32 with DS_EPI_RES_F32) or NULL;
  * out fp16 (fp32 with DS_EPI_OUT_F32).  The sum is exact: results do not depend on the tile shape or on the rows of the launch.  residual
  * may be out itself (the same pointer, type and stride).  The products it stands next to: ds_gemm_f16's dense ones (nn.Linear,
- * attention.py:54-57, 379, 399). */
+ * attention.py:54-57, 379, 399).
+ * workspace: NULL, or at least ds_gemm_i8_workspace_bytes(A, W, desc) bytes at a multiple of 16 -- room for copies of operands whose rows are not
+ * whole multiples of 16 bytes, where those are worth their time (0 where not).  The results are the same with and without. */
+size_t ds_gemm_i8_workspace_bytes(const int8_t* A, const int8_t* W, const ds_gemm_i8_desc* desc);
 int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale, const float* w_scale, const float* bias, const void* residual,
-               void* out, const ds_gemm_i8_desc* desc, void* stream);
+               void* out, const ds_gemm_i8_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 /* h = x + residual; t = h * gamma; root = 1 / sqrt(mean(h^2) + eps) over each row of C values; y = t * root as fp16 / fp32, or (y_dtype
  * DS_I8) q = rint(127 t / max|t|) with scale[row] = max|t| * root / 127.  q is the correctly rounded quotient (halves to even, formed in
  * 64 bits).  residual may be NULL (no addition); sum (NULL: not wanted) receives h in the residual's type, the norm reads the unrounded

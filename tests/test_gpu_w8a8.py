@@ -236,6 +236,16 @@ def test_product_few_rows(m, n, k, act):
     close(run_product(c, act=act), *product_ref(*c, act), F16)
 
 
+@pytest.mark.parametrize("m,n,k", [(2057, 997, 1273), (2057, 1000, 1284), (1500, 1056, 4095)])
+def test_product_with_and_without_copied_operands(m, n, k):
+    """Odd rows laid out anew in the workspace (the usual call) or read as they lie (a call that names its stream has none): the same bits."""
+    (a, w, sa, sw, b, r), (ref, before) = large_case(m, n, k, F32, F32, "none")
+    from dynamicscaler_amd import ops
+    got = ops.gemm_i8(a, w, sa, sw, bias=b, residual=r, out_dtype=F32)
+    assert float(((got.double() - ref).abs() / (before + H32 * (ref.abs() + before))).max()) <= 1.0
+    assert torch.equal(got, ops.gemm_i8(a, w, sa, sw, bias=b, residual=r, out_dtype=F32, stream=torch.cuda.current_stream().cuda_stream))
+
+
 def test_product_is_the_same_for_any_rows_of_the_launch():
     """Row m of a large launch equals the launch of row m alone, bit for bit (every tile shape adds the same exact sum)."""
     a, w, sa, sw, b, _ = product_case(700, 384, 640, 9)
@@ -476,6 +486,18 @@ def test_many_rows(m, n):
     check_rows_i8(q, scale, x.double(), torch.ones(m, 1, dtype=torch.float64))
     v = q.cpu().double() * scale.cpu().double()[:, None]
     close(ops.dequantize_rows_i8(q, scale), v, H32 * v.abs(), F16)
+
+
+def test_more_rows_than_a_launch_has_threads_for():
+    """70 million rows of three values: more workgroups than a grid takes, so each walks several."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    x = torch.randint(-2000, 2001, (70_000_000, 3), device=d, dtype=torch.int16, generator=torch.Generator(device=d).manual_seed(1)).to(F16)
+    q, scale = ops.quantize_rows_i8(x)
+    top = x.float().abs().amax(dim=1, keepdim=True)            # whole numbers below 2^11: 127 x and the quotient's halves are exact in fp32
+    assert torch.equal(q.float(), torch.where(top > 0, torch.round(127 * x.float() / top), torch.zeros_like(top)))
+    y = ops.dequantize_rows_i8(q, scale, dtype=F32)
+    assert torch.equal(y, q.float() * scale[:, None])
 
 
 def test_rows_of_nothing():

@@ -108,14 +108,32 @@ def test_product_c_entry_refuses(fields, args, says):
     for k, v in dict(dict(M=4, N=64, K=32, lda=32, ldw=32, ldc=64, ldr=0, epilogue=0), **fields).items():
         setattr(d, k, v)
     a = dict(dict(A=P, W=P, a_scale=P, w_scale=P, bias=0, residual=0, out=P), **args)
-    refused(_lib.load().ds_gemm_i8(a["A"], a["W"], a["a_scale"], a["w_scale"], a["bias"], a["residual"], a["out"], C.byref(d), 0), says)
+    refused(_lib.load().ds_gemm_i8(a["A"], a["W"], a["a_scale"], a["w_scale"], a["bias"], a["residual"], a["out"], C.byref(d), 0, 0, 0), says)
 
 
 def test_product_c_entry_refuses_no_desc_and_accepts_nothing_to_do():
     lib = _lib.load()
-    refused(lib.ds_gemm_i8(P, P, P, P, 0, 0, P, None, 0), "desc")
+    refused(lib.ds_gemm_i8(P, P, P, P, 0, 0, P, None, 0, 0, 0), "desc")
     d = _lib.GemmI8Desc(M=0, N=64, K=32, lda=32, ldw=32, ldc=64)
-    assert lib.ds_gemm_i8(P, P, P, P, 0, 0, P, C.byref(d), 0) == 0
+    assert lib.ds_gemm_i8(P, P, P, P, 0, 0, P, C.byref(d), 0, 0, 0) == 0
+
+
+def test_product_workspace():
+    """Rows of whole 16s need none; odd ones room for both operands' rows rounded up to 16; a short or crooked one is refused."""
+    lib = _lib.load()
+    d = _lib.GemmI8Desc(M=2057, N=997, K=1280, lda=1280, ldw=1280, ldc=997)
+    assert lib.ds_gemm_i8_workspace_bytes(P, P, C.byref(d)) == 0
+    assert lib.ds_gemm_i8_workspace_bytes(P + 16, P, C.byref(d)) == 0
+    assert lib.ds_gemm_i8_workspace_bytes(P + 4, P, C.byref(d)) == 2057 * 1280
+    assert lib.ds_gemm_i8_workspace_bytes(P, P + 1, C.byref(d)) == 997 * 1280
+    d.K = d.lda = d.ldw = 1273
+    need = lib.ds_gemm_i8_workspace_bytes(P, P, C.byref(d))
+    assert need == (2057 + 997) * 1280
+    refused(lib.ds_gemm_i8(P, P, P, P, 0, 0, P, C.byref(d), P, need - 1, 0), "workspace")
+    refused(lib.ds_gemm_i8(P, P, P, P, 0, 0, P, C.byref(d), P + 8, need, 0), "workspace")
+    d.M = 64                                     # few rows are read as they lie
+    assert lib.ds_gemm_i8_workspace_bytes(P, P, C.byref(d)) == 0
+    assert lib.ds_gemm_i8_workspace_bytes(P, P, None) == 0
 
 
 NORM = dict(x=P, xt=0, ldx=32, r=P, rt=0, ldr=32, g=P, s=P, lds=32, y=P, yt=2, ldy=32, scale=P, rows=4, C=32, eps=1e-6)
