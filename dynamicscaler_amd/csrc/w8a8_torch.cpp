@@ -168,6 +168,8 @@ PyObject* gemm_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
             bias = static_cast<const float*>(b.const_data_ptr());
         }
         const long epilogue = integer(arg[8]);
+        // (the types of `out` and `residual` set the other flags: a flag that says otherwise would write past a buffer)
+        if (epilogue & ~(long)(DS_EPI_GEGLU | DS_EPI_SILU)) refuse("gemm_i8: epilogue " + std::to_string(epilogue) + " is not DS_EPI_GEGLU or DS_EPI_SILU");
         const int64_t cols = epilogue & DS_EPI_GEGLU ? w.m / 2 : w.m;
         ds_gemm_i8_desc d{};
         d.lda = a.ld; d.ldw = w.ld; d.M = (int)a.m; d.N = (int)w.m; d.K = (int)a.n;

@@ -246,12 +246,14 @@ def test_product_with_and_without_copied_operands(m, n, k):
     assert torch.equal(got, ops.gemm_i8(a, w, sa, sw, bias=b, residual=r, out_dtype=F32, stream=torch.cuda.current_stream().cuda_stream))
 
 
-def test_product_is_the_same_for_any_rows_of_the_launch():
-    """Row m of a large launch equals the launch of row m alone, bit for bit (every tile shape adds the same exact sum)."""
-    a, w, sa, sw, b, _ = product_case(700, 384, 640, 9)
-    whole = run_product((a, w, sa, sw, b, None))
+@pytest.mark.parametrize("act", ["none", "silu", "geglu"])
+@pytest.mark.parametrize("out_dtype", [F16, F32])
+def test_product_is_the_same_for_any_rows_of_the_launch(act, out_dtype):
+    """Row m of a large launch equals the launch of row m alone, bit for bit (every kernel adds the same exact sum and ends with the same steps)."""
+    a, w, sa, sw, b, _ = product_case(700, 384, 640, 9, act=act)
+    whole = run_product((a, w, sa, sw, b, None), act=act, out_dtype=out_dtype)
     for lo, hi in ((0, 1), (3, 19), (100, 165), (0, 300), (699, 700)):
-        assert torch.equal(whole[lo:hi], run_product((a[lo:hi], w, sa[lo:hi], sw, b, None)))
+        assert torch.equal(whole[lo:hi], run_product((a[lo:hi], w, sa[lo:hi], sw, b, None), act=act, out_dtype=out_dtype))
 
 
 @pytest.mark.parametrize("which", ["A", "out"])

@@ -37,6 +37,9 @@ def product(**kw):
     (dict(out=torch.zeros((1, 64), dtype=F16).expand(4, 64)), "overlap"),
     (dict(out=torch.zeros((4, 64), dtype=F16), epilogue=DS_EPI_GEGLU), "out.*expected 4 x 32"),
     (dict(out_dtype=torch.bfloat16), "out_dtype"),
+    (dict(epilogue=4), "epilogue 4"),
+    (dict(epilogue=8 | DS_EPI_SILU), "epilogue"),
+    (dict(epilogue=-1), "epilogue"),
     (dict(), "no CPU fallback"),
     (dict(A=[[1]]), "not a tensor"),
 ])
