@@ -83,7 +83,13 @@ __device__ __forceinline__ u32x4 end_chunk(u32x4 v, int k, int K) {
     return u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
 }
 
-__device__ __forceinline__ float silu_f(float v) { return v / (1.0f + expf(-v)); }
+// x / (1 + e^-x) without the divide's ~10 instructions: the hardware's reciprocal (1 ulp) and a Newton step; an infinite denominator gives zero.  For
+// fp16 results the hardware's 2^x and reciprocal as they are (2^-22 and |x| 2^-23 of the value)
+__device__ __forceinline__ float silu_f(float v) {
+    const float d = 1.0f + expf(-v), r = __builtin_amdgcn_rcpf(d);
+    return v * (d < __builtin_huge_valf() ? fmaf(r, fmaf(-d, r, 1.0f), r) : 0.0f);
+}
+__device__ __forceinline__ float silu_f16(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v)); }
 __device__ __forceinline__ float gelu_f(float g) { return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f)); }
 
 // The same for fp16 results: 1 + erf(g / sqrt 2) is E(|g|) for g < 0 and 2 - E(|g|) otherwise, E(a) = erfc(a / sqrt 2) = 2^-q(a) with a polynomial
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__((64 * Few<MT, GEGLU>::WAVES)) gemm_i8_few_kern
         }
         if (!GEGLU && (p.epilogue & DS_EPI_SILU)) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = silu_f(v[j]);
+            for (int j = 0; j < 4; ++j) v[j] = p.epilogue & DS_EPI_OUT_F32 ? silu_f(v[j]) : silu_f16(v[j]);
         }
         if (full) {
             if (p.residual) {
@@ -524,7 +530,7 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         v[j] = scaled(acc[t][RB * b + u][j], sa[RB * b + u], sw[j], bw[j]);
-                        if (p.epilogue & DS_EPI_SILU) v[j] = silu_f(v[j]);
+                        if (p.epilogue & DS_EPI_SILU) v[j] = OUT32 ? silu_f(v[j]) : silu_f16(v[j]);
                     }
                     *reinterpret_cast<f32x4*>(strip + (16 * u + l15) * LD + (OUT32 ? 16 * t + 4 * l4 : 32 * (t >> 1) + 8 * l4 + 4 * (t & 1))) = v;
                 }
@@ -581,7 +587,7 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM
                     const float gate = scaled(acc[t0 + 2 + j / 4][u][j % 4], sa[u], sg[j], bg[j]);
                     v[j] *= OUT32 ? gelu_f(gate) : gelu_f16(gate);
                 } else if (p.epilogue & DS_EPI_SILU) {
-                    v[j] = silu_f(v[j]);
+                    v[j] = OUT32 ? silu_f(v[j]) : silu_f16(v[j]);
                 }
             }
             if (GEGLU || col + CW <= p.N) {

@@ -3,7 +3,8 @@
 Tolerances.  H(t) = half a step of a rounding to t (relative): fp16 2^-11, fp32 2^-24; a subnormal fp16 result is off by at most 2^-25.
   product   p = acc * a_scale * w_scale: the integer sum is exact, its conversion and the two products round (3 H32 |p|), the bias adds one
             rounding of the result (H32 (|p| + |b|)), the residual one more: 5 H32 (|p| + |b| + |r|) in all, then H(out) |out|.
-            SiLU: slope <= 1.1, and x / (1 + e^-x) itself: exp 2 ulp (4 H32), sum, quotient: 8 H32 |silu|.  GEGLU: value * gelu(gate): the
+            SiLU: slope <= 1.1, and x / (1 + e^-x) itself: exp 2 ulp (4 H32), sum, quotient: 8 H32 |silu|; with an fp16 result e^-x is
+            2^(-1.4427 x), whose argument rounds twice (constant and product): 2 H32 |x| |silu| more.  GEGLU: value * gelu(gate): the
             errors of value and gate (slope <= 1.13) are carried, 1 + erf is off by at most 8 H32 absolute, hence gelu by 4 H32 |gate|, and
             three products: 4 H32 |result|.  With an fp16 result gelu comes from a fit of erfc that is within 1.6e-5 of it (found on 200 000 points,
             8.6e-6 ln 2 by the fit and its 32-bit evaluation), the 2^-q within 2e-5: 2e-5 |gate| / 2 erfc(|gate| / sqrt 2) more.
@@ -49,7 +50,7 @@ def product_ref(a, w, sa, sw, bias, residual, act, out=F16):
     v, e = p + b, 5 * H32 * (p.abs() + b.abs())
     if act == "silu":
         s = v * torch.sigmoid(v)
-        e = 1.1 * e + 8 * H32 * s.abs()
+        e = 1.1 * e + 8 * H32 * s.abs() + (2 * H32 * v.abs() * s.abs() if out == F16 else 0.0)
         v = s
     elif act == "geglu":
         m, n = v.shape
