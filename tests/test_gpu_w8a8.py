@@ -207,9 +207,10 @@ def large_case(m, n, k, out_dtype, residual, act, seed=0):
 
 
 # one size for each tile of the many-rows kernel (256 x 256, 128 x 128, 256 x 64, 128 x 64, 64 x 64; 128 x 128 and 64 x 64 through registers), with
-# rows and columns that end inside a tile, the last K-step cut, results below and above the size from which they pass the cache by
+# rows and columns that end inside a tile, the last K-step cut, results below and above the size from which they pass the cache by, a few rows
+# against so many columns that the tiles have them
 @pytest.mark.parametrize("m,n,k", [(8200, 1296, 1040), (16500, 2576, 144), (8200, 2576, 1296), (20500, 656, 336), (40970, 320, 320), (4100, 1296, 1296), (1030, 656, 656),
-                                   (8211, 1297, 1043), (33000, 656, 333), (1030, 657, 655)])
+                                   (8211, 1297, 1043), (33000, 656, 333), (1030, 657, 655), (33, 20480, 656), (50, 4161, 4095)])
 @pytest.mark.parametrize("out_dtype,residual,act", [(F16, None, "none"), (F16, F16, "none"), (F32, F32, "none"), (F32, None, "silu"), (F16, F32, "none"), (F16, None, "geglu"),
                                                     (F32, None, "geglu")])
 def test_product_every_tile(m, n, k, out_dtype, residual, act):
@@ -589,6 +590,18 @@ def test_feed_forward_in_a_graph_and_on_two_streams():
     assert torch.equal(graphs[0][1], feed_forward(p, xs[0], rs[0])[0])
     xs[0].copy_(x0)
     torch.cuda.synchronize()
+    (a, w, sa, sw, b, _), _ = large_case(2057, 997, 1273, F16, None, "none")      # a call with a workspace and a large tile, captured
+    from dynamicscaler_amd import ops
+    ref = ops.gemm_i8(a, w, sa, sw, bias=b)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.gemm_i8(a, w, sa, sw, bias=b)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+        assert torch.equal(ops.gemm_i8(a, w, sa, sw, bias=b), ref)
     streams, outs = [torch.cuda.Stream() for _ in range(2)], [None, None]
     for _ in range(5):
         for i, s in enumerate(streams):
