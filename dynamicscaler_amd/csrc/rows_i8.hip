@@ -203,10 +203,12 @@ __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p
         }
         const double root = NORM ? inverse_root(sum * p.inv_C + (double)p.eps) : 1.0;
         const bool off = I8 && (!(sum < __builtin_huge_val()) || !(top < __builtin_huge_val()));
+        const bool none = off || top == 0.0;              // every q is 0
         // 32-bit quotients v = t (127 / top): t carries two roundings of 2^-24, 127 / top two, v one -- within 3.8e-5 of the quotient, |v| <= 127 --
-        // decide all but the values within 2^-14 of a half (one in 8000); rows whose t or 127 / top are no ordinary fp32 numbers are done exactly
-        const bool in32 = off || top == 0.0 || (top < 1e36 && top > 1e-30);
-        const float inv32 = off || top == 0.0 || !in32 ? 0.0f : 127.0f / (float)top;
+        // decide all but the values within 2^-14 of a half (one in 8000); rows whose h, t or 127 / top are no ordinary fp32 numbers are done exactly
+        // (a small gamma hides an x + r beyond fp32 from top; h^2 <= sum < 1e76 does not)
+        const bool in32 = none || (top < 1e36 && top > 1e-30 && (!RES || sum < 1e76));
+        const float inv32 = none || !in32 ? 0.0f : 127.0f / (float)top;
         double inv = 0.0;
         if (I8 && !in32) inv = 127.0 / top;
         if (I8 && live && lane == 0) p.scale[row] = off ? __builtin_nanf("") : (float)(top * root * (1.0 / 127.0));
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p
                     float t = cx[v].at(j);
                     if constexpr (RES) t += cr[v].at(j);
                     if constexpr (NORM) t *= g[v].at(j);
-                    const float w = off ? 0.0f : t * inv32, n = rintf(w);
+                    const float w = none ? 0.0f : t * inv32, n = rintf(w);
                     q[j] = (int)n;
                     near |= fabsf(w - n) > 0.5f - 0x1p-14f;
                 }

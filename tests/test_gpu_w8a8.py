@@ -419,6 +419,28 @@ def test_norm_of_the_largest_and_smallest_values(n):
     assert bool(back.isinf().all())
 
 
+@pytest.mark.parametrize("n", [5, 64, 320, 1283, 5120, 16384, 20011])
+@pytest.mark.parametrize("gain", [1e-3, 1e-10, 0.0])
+def test_norm_of_sums_beyond_fp32(n, gain):
+    """x + residual leaves fp32 while its product with a small gamma does not: finite inputs, so the rows' 8 bits are the exact quotients (the fp32
+    sum h is infinite there).  Rows of one sign, of both, of a cancelling pair and ordinary ones, for every kernel a row's length chooses."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    big = row_inputs(5, n, n, F32)
+    g = (1.0 + 0.2 * normal((n,), n)) * gain
+    x = big / big.abs().amax(dim=1, keepdim=True) * 3.3e38
+    r = x.clone()
+    x[1], r[1] = x[1].abs(), r[1].abs()
+    r[2] = -x[2] * 0.9999                         # cancels: the sum is ordinary, its parts are not
+    r[3, ::2] = -r[3, ::2]                        # every second sum is zero
+    x[4], r[4] = big[4], 2 * big[4]               # an ordinary row between them
+    h, t, root = rows_ref(x, r, g, 1e-6, True)
+    q, s, back = ops.rmsnorm_i8(x.to(d), g.to(d), residual=r.to(d))
+    check_rows_i8(q, s, t, root)
+    over = h.abs() > torch.finfo(F32).max
+    assert bool(over[:2].any()) and torch.equal(back.cpu().isinf(), over) and bool(s.isfinite().all())
+
+
 @pytest.mark.parametrize("m,n,off", [(5, 320, 8), (5, 320, 3), (4, 641, 1), (3, 5120, 16), (2, 9001, 5)])
 @pytest.mark.parametrize("xt,rt", [(F16, F16), (F16, F32), (F32, F32)])
 def test_rows_strides_and_neighbours(m, n, off, xt, rt):
