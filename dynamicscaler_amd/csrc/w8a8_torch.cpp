@@ -8,7 +8,7 @@
 #include <ATen/ops/empty_cuda_dispatch.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
-#include <cmath>
+#include <optional>
 #include <string>
 #include "../../include/dynscaler_hip.h"
 
@@ -91,19 +91,42 @@ struct Call {
     void with(const at::Tensor& t) const {
         if (t.device() != dev) refuse("tensors on " + dev.str() + " and " + t.device().str() + " in one call");
     }
-    void* stream(PyObject* given) const {
+    void on_current_device() const {
         if (dev.type() != c10::DeviceType::CUDA) refuse("tensors are on " + dev.str() + "; the DynamicScaler hot path has no CPU fallback");
         const int now = c10::hip::current_device();
         if (dev.index() != now)
             refuse("tensors are on " + dev.str() + ", the current device is cuda:" + std::to_string(now) + ": call under torch.cuda.device(" + std::to_string(dev.index()) + ")");
-        if (given == Py_None) return c10::hip::getCurrentHIPStream(dev.index()).stream();
-        void* s = PyLong_AsVoidPtr(given);
-        if (PyErr_Occurred()) throw Raised{};
-        return s;
     }
     at::Tensor empty(at::IntArrayRef sizes, at::ScalarType t) const {
         return at::cuda::empty(sizes, t, c10::kStrided, dev, c10::nullopt, c10::nullopt);
     }
+};
+
+// The stream of a call: the current one, or the one that the caller names by its handle.  A named stream is the current one while the call lasts, so
+// what the call allocates (outputs, workspace) is that stream's, as under torch.cuda.stream(): the allocator hands a block of the stream that
+// was current before to nobody else's kernels, and the other way round.
+class Stream {
+    std::optional<c10::hip::HIPStream> before;
+    hipStream_t handle;
+public:
+    Stream(const Call& call, PyObject* given) {
+        call.on_current_device();
+        const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(call.dev.index());
+        handle = now.stream();
+        if (given == Py_None) return;
+        const uintptr_t named = reinterpret_cast<uintptr_t>(PyLong_AsVoidPtr(given));
+        if (PyErr_Occurred()) throw Raised{};
+        handle = reinterpret_cast<hipStream_t>(named);
+        if (handle == now.stream()) return;
+        before = now;                         // (1 is the default stream's other name; odd numbers mean pool streams to torch)
+        c10::hip::setCurrentHIPStream(c10::hip::getStreamFromExternal(reinterpret_cast<hipStream_t>(named & 1 ? 0 : named), call.dev.index()));
+    }
+    ~Stream() {
+        if (before) c10::hip::setCurrentHIPStream(*before);
+    }
+    Stream(const Stream&) = delete;
+    Stream& operator=(const Stream&) = delete;
+    operator void*() const { return handle; }
 };
 
 void done(int rc, const char* what) {
@@ -190,15 +213,14 @@ PyObject* gemm_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
         }
         const at::ScalarType type = out.defined() ? out.scalar_type() : rows_type(arg[7], "gemm_i8: out_dtype");
         if (type == at::kFloat) d.epilogue |= DS_EPI_OUT_F32;
-        void* st = call.stream(arg[9]);
+        const Stream st(call, arg[9]);
         if (!out.defined()) {
             out = call.empty({a.m, cols}, type);
             d.ldc = cols;
         }
         const int8_t *pa = static_cast<const int8_t*>(A.const_data_ptr()), *pw = static_cast<const int8_t*>(W.const_data_ptr());
-        // the workspace goes back to the allocator with the call, so it is one of the current stream's: a call that names another does without
-        at::Tensor room;
-        const size_t bytes = arg[9] == Py_None ? c_gemm_workspace(pa, pw, &d) : 0;
+        at::Tensor room;                       // back to the allocator with the call: the next block of the same stream
+        const size_t bytes = c_gemm_workspace(pa, pw, &d);
         if (bytes) room = call.empty({(int64_t)bytes}, at::kChar);
         done(c_gemm(pa, pw, static_cast<const float*>(sa.const_data_ptr()), static_cast<const float*>(sw.const_data_ptr()), bias, residual, out.data_ptr(), &d,
                     bytes ? room.data_ptr() : nullptr, bytes, st), "ds_gemm_i8");
@@ -248,7 +270,7 @@ PyObject* rmsnorm(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
             call.with(*given_scale);
             scale = *given_scale;
         }
-        void* st = call.stream(arg[10]);
+        const Stream st(call, arg[10]);
         if (res && !sum.defined()) {
             sum = call.empty({r.m, r.n}, res->scalar_type());
             d.lds = r.n;
@@ -285,7 +307,7 @@ PyObject* quantize_rows_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
             vector_of(scale, {op, "scale"}, r.m);
             call.with(scale);
         }
-        void* st = call.stream(arg[3]);
+        const Stream st(call, arg[3]);
         if (!q.defined()) q = call.empty({r.m, r.n}, at::kChar);
         if (!scale.defined()) scale = call.empty({r.m}, at::kFloat);
         done(c_quantize(x.const_data_ptr(), ds_type(x), r.ld, static_cast<int8_t*>(q.data_ptr()), ldq, static_cast<float*>(scale.data_ptr()), (int)r.m, (int)r.n, st), "ds_quantize_rows_i8");
@@ -311,7 +333,7 @@ PyObject* dequantize_rows_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) 
             call.with(y);
         }
         const at::ScalarType type = y.defined() ? y.scalar_type() : rows_type(arg[3], "dequantize_rows_i8: dtype");
-        void* st = call.stream(arg[4]);
+        const Stream st(call, arg[4]);
         if (!y.defined()) y = call.empty({r.m, r.n}, type);
         done(c_dequantize(static_cast<const int8_t*>(q.const_data_ptr()), r.ld, static_cast<const float*>(scale.const_data_ptr()), y.data_ptr(), ds_type(y), ldy, (int)r.m, (int)r.n, st),
              "ds_dequantize_rows_i8");

@@ -548,7 +548,8 @@ def temporal_attention(q, k, v, out, *, nseq_batches, T, hw, heads, ldq, ldk, ld
 # ------------------------------------------------------------------------------------------------ W8A8
 # The checks, the outputs' allocation and the call are C++ (csrc/w8a8_torch.cpp): on a few rows the host's share of a call is longer than the
 # kernel.  Every function takes 2-D tensors with contiguous columns and any row stride that keeps rows apart, all on the current device, and
-# raises DsError for anything else.
+# raises DsError for anything else.  `stream` is a HIP stream's handle (None: the current stream): the call runs on it, and what the call allocates
+# belongs to it, as under torch.cuda.stream().
 _W8A8 = None
 
 

@@ -634,6 +634,96 @@ def test_feed_forward_in_a_graph_and_on_two_streams():
         assert torch.equal(got, ref)
 
 
+def calls_that_allocate(d):
+    """Each operator as a call without outputs, keyword arguments to come; the product with odd rows, which it lays out anew in a workspace."""
+    from dynamicscaler_amd import ops
+    (a, w, sa, sw, b, r), _ = large_case(2057, 997, 1273, F32, F32, "none")
+    x, g, res = normal((301, 1283), 1, F16).to(d), normal((1283,), 2).to(d), normal((301, 1283), 3).to(d)
+    q, s = ops.quantize_rows_i8(x)
+    return {"product": lambda **kw: (ops.gemm_i8(a, w, sa, sw, bias=b, residual=r, out_dtype=F32, **kw),),
+            "norm": lambda **kw: ops.rmsnorm(x, g, residual=res, **kw),
+            "norm_i8": lambda **kw: ops.rmsnorm_i8(x, g, residual=res, **kw),
+            "quantize": lambda **kw: ops.quantize_rows_i8(x, **kw),
+            "dequantize": lambda **kw: (ops.dequantize_rows_i8(q, s, **kw),)}
+
+
+@pytest.mark.parametrize("which", ["product", "norm", "norm_i8", "quantize", "dequantize"])
+def test_outputs_of_a_call_on_a_named_stream_belong_to_it(which):
+    """A block that the current stream gave back is still its own (kernels in flight may use it): the outputs of a call on another stream are
+    other blocks, and come back to that stream.  The results are the same, captured ones too, and the current stream stays what it was."""
+    d = dev()
+    call = calls_that_allocate(d)[which]
+    ref = call()
+    side, here = torch.cuda.Stream(), torch.cuda.current_stream()
+    torch.cuda.synchronize()
+    blocks = [torch.empty_like(t) for t in ref]
+    theirs = {t.data_ptr() for t in blocks}
+    del blocks
+    outs = call(stream=side.cuda_stream)
+    assert torch.cuda.current_stream() == here
+    side.synchronize()
+    assert not theirs & {t.data_ptr() for t in outs}
+    assert all(torch.equal(a, b) for a, b in zip(outs, ref))
+    again = call(stream=here.cuda_stream)
+    here.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, ref))
+    mine = {t.data_ptr() for t in outs}
+    del outs
+    blocks = [torch.empty_like(t) for t in ref]
+    assert not mine & {t.data_ptr() for t in blocks}
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        side.wait_stream(torch.cuda.current_stream())
+        outs = call(stream=side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        for t in outs:
+            t.zero_()
+        g.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(outs, ref, eager))
+
+
+def test_products_with_a_workspace_on_two_streams():
+    """Each call's workspace is its own stream's: two at once, the current stream's and a named one's, do not meet."""
+    from dynamicscaler_amd import ops
+    cases = [large_case(2057, 997, 1273, F16, None, "none", seed)[0] for seed in (1, 2)]
+    refs = [ops.gemm_i8(a, w, sa, sw, bias=b) for a, w, sa, sw, b, _ in cases]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        for (a, w, sa, sw, b, _), stream in zip(cases, (None, side.cuda_stream)):
+            outs.append(ops.gemm_i8(a, w, sa, sw, bias=b, stream=stream))
+    torch.cuda.synchronize()
+    for i, got in enumerate(outs):
+        assert torch.equal(got, refs[i % 2])
+
+
+@pytest.mark.parametrize("m,n,k", [(2057, 997, 1273), (2057, 1000, 1284), (1500, 1056, 4095)])
+@pytest.mark.parametrize("flags", [0, 4, 2, 2 | 4 | 8])
+def test_product_c_entry_without_a_workspace(m, n, k, flags):
+    """The C entry with and without room for aligned copies, SiLU in front of a residual among the flags (the tensor front end's calls always
+    bring the room that helps): the same bits, and right."""
+    import ctypes as C
+    from dynamicscaler_amd import _lib
+    out_dtype, residual = (F32 if flags & 4 else F16), (F32 if flags & 8 else F16)
+    act = "silu" if flags & 2 else "none"
+    (a, w, sa, sw, b, r), (ref, before) = large_case(m, n, k, out_dtype, residual, act)
+    lib, st, outs = _lib.load(), torch.cuda.current_stream().cuda_stream, []
+    desc = _lib.GemmI8Desc(lda=k, ldw=k, ldc=n, ldr=n, M=m, N=n, K=k, epilogue=flags)
+    need = lib.ds_gemm_i8_workspace_bytes(a.data_ptr(), w.data_ptr(), C.byref(desc))
+    assert need > 0
+    room = torch.empty(need, dtype=torch.uint8, device=a.device)
+    for at, size in ((0, 0), (room.data_ptr(), need)):
+        outs.append(torch.empty((m, n), dtype=out_dtype, device=a.device))
+        assert lib.ds_gemm_i8(a.data_ptr(), w.data_ptr(), sa.data_ptr(), sw.data_ptr(), b.data_ptr(), r.data_ptr(), outs[-1].data_ptr(), C.byref(desc), at, size, st) == 0
+    assert torch.equal(*outs)
+    off = (outs[0].double() - ref).abs()
+    assert float((off / (before + HALF[out_dtype] * (ref.abs() + before) + SUB[out_dtype])).max()) <= 1.0
+
+
 def test_timing_hook_sees_the_product():
     from dynamicscaler_amd import ops
     seen = []
