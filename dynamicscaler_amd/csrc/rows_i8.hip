@@ -73,6 +73,13 @@ typedef f32x4 __attribute__((aligned(4))) f32x4_u;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 __attribute__((aligned(1))) u32x2_u;
 
+// v + lost (v rounded to nearest, `lost` what the rounding took away) rounded to odd: towards zero, and the last bit set where that lost anything.  What
+// goes on to fp16 from there is rounded once in effect (von Neumann's rounding: fp32 has the two spare bits that it needs).
+__device__ __forceinline__ float to_odd(float v, float lost) {
+    const unsigned u = __float_as_uint(v), towards_zero = (int)(__float_as_uint(lost) ^ u) >> 31;
+    return fabsf(lost) > 0.0f ? __uint_as_float((u + towards_zero) | 1) : v;        // (no for the NaN that an infinite v leaves)
+}
+
 template <typename T> struct Chunk;
 template <> struct Chunk<f16> {
     f16x8 v;
@@ -310,10 +317,10 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p, int rows) {
 }
 
 // The chunks of 8 values of all rows in one sequence, `span` of them a workgroup (per_row of them a row; magic: i / per_row = i * magic >> 40 for
-// i < per_row + span, both < 2^16): every lane has work whatever the row's length.  C >= 8; a row's last chunk ends at the row's end.  655360 x 320 to fp16 97 us (6.5 TB/s); with
-// teams of 64 lanes a row, 40 of them at work, 186 us.
+// i < per_row + span, both < 2^16): every lane has work whatever the row's length.  C >= 8; a row's last chunk ends at the row's end.  655360 x 320 to fp16 110 us (5.7 TB/s; with
+// a second rounding in place of the odd one 108), with teams of 64 lanes a row, 40 of them at work, 186 us before that.
 template <typename Y>
-__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C,
+__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__ q8, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C,
                                                       unsigned per_row, unsigned long long magic, int span) {
     const unsigned long long first = (unsigned long long)blockIdx.x * span;
     const long row0 = first / per_row;
@@ -325,10 +332,13 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__
         if (row >= rows) break;
         const int c = min((int)(i - r * per_row) * 8, C - 8);
         const float s = scale[row];
-        const u32x2 v = *reinterpret_cast<const u32x2_u*>(q + row * ldq + c);
+        const u32x2 v = *reinterpret_cast<const u32x2_u*>(q8 + row * ldq + c);
         Chunk<Y> cy;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) cy.set(j, (float)((int)(v[j >> 2] << (24 - 8 * (j & 3))) >> 24) * s);
+        for (int j = 0; j < 8; ++j) {
+            const float q = (float)((int)(v[j >> 2] << (24 - 8 * (j & 3))) >> 24), p = q * s;
+            cy.set(j, sizeof(Y) == 2 ? to_odd(p, fmaf(q, s, -p)) : p);
+        }
         cy.store(y + row * ldy + c);
     }
 }
@@ -338,7 +348,7 @@ template <typename Y>
 __global__ void __launch_bounds__(256) dequant_any_kernel(const int8_t* __restrict__ q, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C) {
     for (long row = blockIdx.x; row < rows; row += gridDim.x) {
         const float s = scale[row];
-        for (int c = threadIdx.x; c < C; c += blockDim.x) y[row * ldy + c] = (Y)((float)q[row * ldq + c] * s);
+        for (int c = threadIdx.x; c < C; c += blockDim.x) y[row * ldy + c] = (Y)((double)q[row * ldq + c] * (double)s);
     }
 }
 

@@ -344,6 +344,28 @@ def test_quantize_and_back(m, n, xt):
     assert bool(((y.double().cpu() - x.double()).abs() <= scale.cpu().double()[:, None] * (0.5 + 1e-4)).all())
 
 
+def once(v):
+    """fp64 to fp16 in one rounding (torch goes by way of fp32)."""
+    import numpy as np
+    with np.errstate(over="ignore"):
+        return torch.from_numpy(v.numpy().astype(np.float16))
+
+
+@pytest.mark.parametrize("m,n", [(20000, 3), (5000, 320), (301, 1283)])
+@pytest.mark.parametrize("size", [1.0, 1e-5, 400.0, 2000.0, 3e38])
+def test_dequantize_rounds_once(m, n, size):
+    """fp16 results are the products' own roundings, bit for bit: an fp32 product that lands on the half between two fp16 values decides nothing
+    (one value in 16000; `size` brings subnormal results and infinite ones in)."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    q = ints((m, n), m)
+    s = torch.rand(m, generator=gen(n)) * size
+    v = q.double() * s.double()[:, None]
+    assert bool((once(v) != v.float().to(F16)).any()) or m * n < 10 ** 6 or size > 1e4              # there are such values among them
+    assert torch.equal(ops.dequantize_rows_i8(q.to(d), s.to(d)).cpu(), once(v))
+    assert torch.equal(ops.dequantize_rows_i8(q.to(d), s.to(d), dtype=F32).cpu(), v.float())
+
+
 @pytest.mark.parametrize("xt", [F16, F32])
 def test_quantize_halves_go_to_even(xt):
     """Quotients that are exact halves (63.5 at x = max / 2; a row whose steps are whole numbers), and their neighbours one ulp away."""
