@@ -7,6 +7,7 @@
 // t is formed and compared in 64 bits and the sums are 64-bit, so q is the correctly rounded quotient (halves to even) of the inputs as
 // they are given: it does not depend on the order of a reduction.  A row without a largest value (all zeros) has q = 0, scale = 0; a row that
 // holds a NaN or an infinity (in x, r or t) has q = 0, scale = NaN: it stands for NaN throughout.
+// fp16 results are rounded once, from the 64-bit value (by way of a rounding to odd: fp16 rows of 655360 x 320 164 us, 159 with two roundings).
 #include "common.h"
 
 namespace {
@@ -79,6 +80,11 @@ __device__ __forceinline__ float to_odd(float v, float lost) {
     const unsigned u = __float_as_uint(v), towards_zero = (int)(__float_as_uint(lost) ^ u) >> 31;
     return fabsf(lost) > 0.0f ? __uint_as_float((u + towards_zero) | 1) : v;        // (no for the NaN that an infinite v leaves)
 }
+// the same for 64 bits, to the 21 that the upper word holds (and fp32 takes as they are)
+__device__ __forceinline__ double to_odd(double v) {
+    const unsigned long long u = __double_as_longlong(v);
+    return __longlong_as_double((unsigned long long)((unsigned)(u >> 32) | min((unsigned)u, 1u)) << 32);
+}
 
 template <typename T> struct Chunk;
 template <> struct Chunk<f16> {
@@ -87,7 +93,8 @@ template <> struct Chunk<f16> {
     __device__ __forceinline__ void load(const f16* p) { v = *reinterpret_cast<const f16x8_u*>(p); }
     __device__ __forceinline__ void hold() { asm volatile("" : "+v"(v)); }
     __device__ __forceinline__ float at(int j) const { return (float)v[j]; }
-    __device__ __forceinline__ void set(int j, double x) { v[j] = (f16)(float)x; }
+    __device__ __forceinline__ void set(int j, float x) { v[j] = (f16)x; }
+    __device__ __forceinline__ void set(int j, double x) { set(j, (float)to_odd(x)); }
     __device__ __forceinline__ void store(f16* p) const { *reinterpret_cast<f16x8_u*>(p) = v; }
 };
 template <> struct Chunk<float> {
@@ -99,7 +106,8 @@ template <> struct Chunk<float> {
         v[1] = *reinterpret_cast<const f32x4_u*>(p + 4);
     }
     __device__ __forceinline__ float at(int j) const { return v[j >> 2][j & 3]; }
-    __device__ __forceinline__ void set(int j, double x) { v[j >> 2][j & 3] = (float)x; }
+    __device__ __forceinline__ void set(int j, float x) { v[j >> 2][j & 3] = x; }
+    __device__ __forceinline__ void set(int j, double x) { set(j, (float)x); }
     __device__ __forceinline__ void store(float* p) const {
         *reinterpret_cast<f32x4_u*>(p) = v[0];
         *reinterpret_cast<f32x4_u*>(p + 4) = v[1];
@@ -259,7 +267,11 @@ __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p
             if constexpr (RES) {
                 Chunk<R> ch;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ch.set(j, cx[v].at(j) + cr[v].at(j));
+                for (int j = 0; j < 8; ++j) {
+                    // (the fp32 sum of two fp16 values is exact wherever it is near a half of fp16)
+                    if constexpr (sizeof(X) == 4 && sizeof(R) == 2) ch.set(j, h_of(v, j));
+                    else ch.set(j, cx[v].at(j) + cr[v].at(j));
+                }
                 if (mine && p.h) ch.store(hs + at(v));
             }
         }
@@ -309,7 +321,7 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p, int rows) {
             Y* y = reinterpret_cast<Y*>(p.y) + row * p.ldy;
             for (int c = tid; c < p.C; c += blockDim.x) {
                 const double h = h_of(c);
-                y[c] = (Y)(float)(h * root * (double)p.g[c]);
+                y[c] = (Y)(h * (double)p.g[c] * root);
                 if (p.h) reinterpret_cast<R*>(p.h)[row * p.ldh + c] = (R)h;
             }
         }

@@ -364,7 +364,7 @@ int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale, const flo
 /* h = x + residual; t = h * gamma; root = 1 / sqrt(mean(h^2) + eps) over each row of C values; y = t * root as fp16 / fp32, or (y_dtype
  * DS_I8) q = rint(127 t / max|t|) with scale[row] = max|t| * root / 127.  q is the correctly rounded quotient (halves to even, formed in
  * 64 bits).  residual may be NULL (no addition); sum (NULL: not wanted) receives h in the residual's type, the norm reads the unrounded
- * h.  8-bit rows: all t zero -> q = 0, scale = 0; a NaN or an infinity in the row -> q = 0, scale = NaN.  eps > 0.
+ * h; y and sum are rounded once.  8-bit rows: all t zero -> q = 0, scale = 0; a NaN or an infinity in the row -> q = 0, scale = NaN.  eps > 0.
  * In place: sum may be residual, and a fp16 / fp32 y may be x (same type and stride). */
 typedef struct ds_rmsnorm_desc {
     int64_t ldx, ldr, lds, ldy;               /* row strides of x, residual, sum and y in elements              */

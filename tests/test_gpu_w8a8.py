@@ -366,6 +366,25 @@ def test_dequantize_rounds_once(m, n, size):
     assert torch.equal(ops.dequantize_rows_i8(q.to(d), s.to(d), dtype=F32).cpu(), v.float())
 
 
+@pytest.mark.parametrize("m,n", [(400000, 5), (5000, 320), (1501, 1283), (100, 20011)])
+@pytest.mark.parametrize("xt,rt", [(F32, F16), (F16, F16), (F16, F32), (F32, None)])
+@pytest.mark.parametrize("size", [1.0, 2e-5, 300.0])
+def test_norm_rounds_once(m, n, xt, rt, size):
+    """The fp16 sum and the fp16 result are single roundings of the 64-bit ones.  The result's root is within 2^-44 of itself: values that close
+    to a half between two fp16 values are left out (2^-40: one in 10^8)."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    x, g = row_inputs(m, n, m + 7, F32).mul(size).to(xt), (1.0 + 0.2 * normal((n,), n)) * size
+    r = None if rt is None else normal((m, n), m, rt, size)
+    h, t, root = rows_ref(x, r, g, 1e-6, True)
+    y, back = ops.rmsnorm(x.to(d), g.to(d), residual=None if r is None else r.to(d))
+    v = t * root
+    sure = once(v * (1 + 2.0 ** -40)) == once(v * (1 - 2.0 ** -40))
+    assert bool(((y.cpu() == once(v)) | ~sure).all()) and float(sure.float().mean()) > 0.999
+    if rt is not None:
+        assert torch.equal(back.cpu(), once(h) if rt == F16 else h.float())
+
+
 @pytest.mark.parametrize("xt", [F16, F32])
 def test_quantize_halves_go_to_even(xt):
     """Quotients that are exact halves (63.5 at x = max / 2; a row whose steps are whole numbers), and their neighbours one ulp away."""
