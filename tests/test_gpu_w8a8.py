@@ -117,6 +117,31 @@ def test_product_activations(m, n, k, act, out_dtype, bias):
     close(got, *product_ref(*c, act, out_dtype), out_dtype)
 
 
+@pytest.mark.parametrize("m,k", [(2, 64), (40, 100), (300, 64), (300, 37), (2500, 64)])
+def test_geglu_of_far_gates(m, k):
+    """fp32 GEGLU relative to itself for gates down to where erfc leaves fp32: operands whose sums are one and whose scales are the values and gates,
+    so that both are exact.  E = erfc(|gate| / sqrt 2) is off by at most 12 H32 E (8 in the formula's own roundings, 4 for the hardware's reciprocal and
+    power of two), value * gate / 2 * (E or 2 - E) rounds four times, the result once."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    groups = 64
+    gates = torch.cat([torch.linspace(-12.9, 12.9, 32 * groups - 32), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-6, -1e-6, -5.5, -6.0] * 4)])
+    gates = gates[torch.randperm(32 * groups, generator=gen(1))].view(groups, 32)
+    values = (0.5 + 1.5 * torch.rand((groups, 32), generator=gen(2)))
+    values[::3] *= 1e6
+    a, w = torch.zeros((m, k), dtype=torch.int8), torch.zeros((64 * groups, k), dtype=torch.int8)
+    a[:, k - 1] = 1
+    w[:, k - 1] = 1
+    sw = torch.stack([values, gates], dim=1).reshape(-1)
+    got = ops.gemm_i8(a.to(d), w.to(d), torch.ones(m, device=d), sw.to(d), out_dtype=F32, epilogue=EPI["geglu"]).cpu()
+    g = gates.double()
+    ref = (values.double() * g / 2 * torch.erfc(-g / math.sqrt(2.0))).reshape(1, -1).expand(m, -1)
+    e = torch.erfc(g.abs() / math.sqrt(2.0))
+    factor = torch.where(g < 0, e, 2 - e)
+    before = (12 * e / factor + 4).reshape(1, -1) * H32 * ref.abs()
+    close(got, ref, before, F32)
+
+
 @pytest.mark.parametrize("m,n,k", [(4, 40, 131071), (130, 70, 131071), (260, 256, 131056)])
 def test_product_longest_sums_are_exact(m, n, k):
     """Every term 2^14: the sums reach 2^31 - 2^14 and have to come out whole (fp32 out, scales of one)."""
