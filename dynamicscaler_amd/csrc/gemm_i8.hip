@@ -502,21 +502,22 @@ __global__ void __launch_bounds__((I8Tile<BM, BN, WGM, WGN, NS>::NT), (DMA || BM
             else v[j] += (float)__builtin_bit_cast(f16x2, (unsigned)r[j / 4][(j % 4) / 2])[j % 2];
         }
     };
-    // STREAM (results that L2 does not hold): past the cache, A rows and W panels stay (16384 x 2560 x 1280 in fp16: 85 -> 66 us)
-    auto store = [](auto v, auto* to) {
-        if constexpr (STREAM) __builtin_nontemporal_store(v, to);
-        else *to = v;
-    };
+    // STREAM (results that L2 does not hold): past the cache, A rows and W panels stay (16384 x 2560 x 1280 in fp16: 85 -> 66 us).  The pointers say
+    // that a row may begin at any element.
     auto store_columns = [&](int m, int col, const float* v) {
         const long at = (long)m * p.ldc + col;
         if constexpr (OUT32) {
             const f32x4 o = {v[0], v[1], v[2], v[3]};
-            store(o, reinterpret_cast<f32x4_u*>(reinterpret_cast<float*>(p.out) + at));
+            f32x4_u* to = reinterpret_cast<f32x4_u*>(reinterpret_cast<float*>(p.out) + at);
+            if constexpr (STREAM) __builtin_nontemporal_store(o, to);
+            else *to = o;
         } else {
             f16x8 h;
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
-            store(h, reinterpret_cast<f16x8_u*>(reinterpret_cast<f16*>(p.out) + at));
+            f16x8_u* to = reinterpret_cast<f16x8_u*>(reinterpret_cast<f16*>(p.out) + at);
+            if constexpr (STREAM) __builtin_nontemporal_store(h, to);
+            else *to = h;
         }
     };
     float sa[TM];

@@ -2,6 +2,7 @@
 import ctypes as C
 import os
 import re
+import subprocess
 
 import pytest
 import torch
@@ -175,3 +176,14 @@ def test_desc_layout_matches_the_header(name, cls):
     body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), header, flags=re.S).group(1)
     fields = [(n.strip(), t) for t, names in re.findall(r"(int32_t|int64_t|float) ([^;]+);", body) for n in names.split(",")]
     assert [(n, {C.c_int64: "int64_t", C.c_int32: "int32_t", C.c_float: "float"}[t]) for n, t in cls._fields_] == fields
+
+
+@pytest.mark.parametrize("source", ["gemm_i8.hip", "rows_i8.hip"])
+def test_sources_compile_without_warnings(source):
+    """Among them -Walign-mismatch: loads and stores at any element are declared so, whatever the hardware accepts."""
+    from dynamicscaler_amd import build
+    if not os.path.exists(build.HIPCC):
+        pytest.skip("needs hipcc")
+    r = subprocess.run([build.HIPCC] + build.FLAGS + build.SOURCE_FLAGS[source] + ["-Werror", "-Wno-unused-command-line-argument", "--cuda-device-only", "-fsyntax-only",
+                                                                                   "-x", "hip", os.path.join(build.CSRC, source)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
