@@ -198,13 +198,14 @@ def load_w8a8():
     """The W8A8 operators' tensor front end (csrc/w8a8_torch.cpp), bound to the entries of the loaded library."""
     global _w8a8
     if _w8a8 is None:
+        import torch
         lib = load()
         try:
             from . import _w8a8 as front
         except ImportError as e:
             raise HipLibraryMissing(f"cannot load {os.path.join(HERE, '_w8a8.so')}: build it with `python -m dynamicscaler_amd.build` ({e})") from e
-        front.bind(DsError, *(C.cast(f, C.c_void_p).value for f in (lib.ds_gemm_i8_workspace_bytes, lib.ds_gemm_i8, lib.ds_rmsnorm_rows,
-                                                                  lib.ds_quantize_rows_i8, lib.ds_dequantize_rows_i8, lib.ds_last_error)))
+        entries = (lib.ds_gemm_i8_workspace_bytes, lib.ds_gemm_i8, lib.ds_rmsnorm_rows, lib.ds_quantize_rows_i8, lib.ds_dequantize_rows_i8, lib.ds_last_error)
+        front.bind(DsError, torch.OutOfMemoryError, *(C.cast(f, C.c_void_p).value for f in entries))
         _w8a8 = front
     return _w8a8
 

@@ -20,7 +20,7 @@ decltype(&ds_rmsnorm_rows) c_rmsnorm;
 decltype(&ds_quantize_rows_i8) c_quantize;
 decltype(&ds_dequantize_rows_i8) c_dequantize;
 decltype(&ds_last_error) c_last_error;
-PyObject* ds_error = nullptr;
+PyObject *ds_error = nullptr, *out_of_memory = nullptr;
 
 struct Refused { std::string says; };
 struct Raised {};                      // a Python error is set
@@ -164,7 +164,7 @@ template <typename F> PyObject* guarded(Py_ssize_t n, Py_ssize_t expected, F&& f
         PyErr_SetString(ds_error, r.says.c_str());
     } catch (const Raised&) {
     } catch (const c10::OutOfMemoryError& e) {
-        PyErr_SetString(PyExc_MemoryError, e.what_without_backtrace());
+        PyErr_SetString(out_of_memory, e.what_without_backtrace());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     }
@@ -341,11 +341,11 @@ PyObject* dequantize_rows_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) 
     });
 }
 
-// the exception class and the entries' addresses (gemm's workspace, gemm, rmsnorm, quantize, dequantize, last_error)
+// the classes of refusals and of failed allocations, and the entries' addresses (gemm's workspace, gemm, rmsnorm, quantize, dequantize, last_error)
 PyObject* bind(PyObject*, PyObject* args) {
-    PyObject* cls;
+    PyObject *cls, *oom;
     unsigned long long f[6];
-    if (!PyArg_ParseTuple(args, "OKKKKKK", &cls, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5])) return nullptr;
+    if (!PyArg_ParseTuple(args, "OOKKKKKK", &cls, &oom, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5])) return nullptr;
     c_gemm_workspace = reinterpret_cast<decltype(c_gemm_workspace)>(f[0]);
     c_gemm = reinterpret_cast<decltype(c_gemm)>(f[1]);
     c_rmsnorm = reinterpret_cast<decltype(c_rmsnorm)>(f[2]);
@@ -353,8 +353,11 @@ PyObject* bind(PyObject*, PyObject* args) {
     c_dequantize = reinterpret_cast<decltype(c_dequantize)>(f[4]);
     c_last_error = reinterpret_cast<decltype(c_last_error)>(f[5]);
     Py_INCREF(cls);
+    Py_INCREF(oom);
     Py_XDECREF(ds_error);
+    Py_XDECREF(out_of_memory);
     ds_error = cls;
+    out_of_memory = oom;
     Py_RETURN_NONE;
 }
 

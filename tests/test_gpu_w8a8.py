@@ -12,6 +12,7 @@ Tolerances.  H(t) = half a step of a rounding to t (relative): fp16 2^-11, fp32 
   norm y    h, root, gamma: at most five fp32 roundings (5 H32) before H(out).
   sum       H32 + H(out).
 """
+import contextlib
 import math
 
 import pytest
@@ -788,6 +789,35 @@ def test_product_c_entry_without_a_workspace(m, n, k, flags):
     assert torch.equal(*outs)
     off = (outs[0].double() - ref).abs()
     assert float((off / (before + HALF[out_dtype] * (ref.abs() + before) + SUB[out_dtype])).max()) <= 1.0
+
+
+@contextlib.contextmanager
+def at_most(mib):
+    """The allocator may take `mib` MiB more than what is held now."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (mib << 20)) / torch.cuda.get_device_properties(0).total_memory)
+    try:
+        yield
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+def test_outputs_that_do_not_fit_raise_as_everywhere():
+    """torch.OutOfMemoryError, as the other operators' allocations do; the same call goes through once there is room."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    x, g = torch.ones((50000, 2048), dtype=F16, device=d), torch.ones(2048, device=d)
+    q, s = ops.quantize_rows_i8(x)
+    calls = [lambda: ops.gemm_i8(q, q[:2048], s, s[:2048]), lambda: ops.rmsnorm(x, g), lambda: ops.rmsnorm_i8(x, g), lambda: ops.quantize_rows_i8(x),
+             lambda: ops.dequantize_rows_i8(q, s)]
+    with at_most(16):
+        for call in calls:
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
 
 
 def test_timing_hook_sees_the_product():
