@@ -221,9 +221,14 @@ PyObject* gemm_i8(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
         const int8_t *pa = static_cast<const int8_t*>(A.const_data_ptr()), *pw = static_cast<const int8_t*>(W.const_data_ptr());
         at::Tensor room;                       // back to the allocator with the call: the next block of the same stream
         const size_t bytes = c_gemm_workspace(pa, pw, &d);
-        if (bytes) room = call.empty({(int64_t)bytes}, at::kChar);
+        if (bytes) {
+            try {
+                room = call.empty({(int64_t)bytes}, at::kChar);
+            } catch (const c10::OutOfMemoryError&) {      // slower without
+            }
+        }
         done(c_gemm(pa, pw, static_cast<const float*>(sa.const_data_ptr()), static_cast<const float*>(sw.const_data_ptr()), bias, residual, out.data_ptr(), &d,
-                    bytes ? room.data_ptr() : nullptr, bytes, st), "ds_gemm_i8");
+                    room.defined() ? room.data_ptr() : nullptr, room.defined() ? bytes : 0, st), "ds_gemm_i8");
         return handed(arg[6], out);
     });
 }

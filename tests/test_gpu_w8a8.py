@@ -820,6 +820,21 @@ def test_outputs_that_do_not_fit_raise_as_everywhere():
     torch.cuda.synchronize()
 
 
+def test_product_without_room_for_its_workspace():
+    """The workspace only makes odd rows quicker: where it cannot be had the call reads them as they lie, with the same bits."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    a, w, sa, sw, b, _ = [None if t is None else t.to(d) for t in product_case(20057, 1997, 1273, 5)]
+    ref = ops.gemm_i8(a, w, sa, sw, bias=b)
+    out = torch.zeros_like(ref)
+    with at_most(2):                              # (28 MB of copies)
+        with pytest.raises(torch.OutOfMemoryError):
+            torch.empty((20057 + 1997) * 1280, dtype=torch.int8, device=d)
+        ops.gemm_i8(a, w, sa, sw, bias=b, out=out)
+        torch.cuda.synchronize()
+    assert torch.equal(out, ref)
+
+
 def test_timing_hook_sees_the_product():
     from dynamicscaler_amd import ops
     seen = []
