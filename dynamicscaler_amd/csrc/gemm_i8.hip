@@ -789,8 +789,19 @@ int launch_i8(const I8Args& p, bool dma, bool odd, hipStream_t st) {
 
 }  // namespace
 
+// what makes a product of these sizes illegal whatever its operands
+static int check_desc(const ds_gemm_i8_desc& d) {
+    DS_CHECK_ARG(d.M >= 0 && d.N >= 0 && d.K >= 0, "ds_gemm_i8: negative size (M %d, N %d, K %d)", d.M, d.N, d.K);
+    DS_CHECK_ARG(d.K <= 131071, "ds_gemm_i8: K %d: the 32-bit sums hold K <= 131071", d.K);
+    DS_CHECK_ARG((d.epilogue & ~(DS_EPI_GEGLU | DS_EPI_SILU | DS_EPI_OUT_F32 | DS_EPI_RES_F32)) == 0, "ds_gemm_i8: epilogue %d", d.epilogue);
+    const bool geglu = d.epilogue & DS_EPI_GEGLU;
+    DS_CHECK_ARG(!(geglu && (d.epilogue & DS_EPI_SILU)), "ds_gemm_i8: GEGLU and SiLU exclude each other");
+    DS_CHECK_ARG(!geglu || d.N % 64 == 0, "ds_gemm_i8: GEGLU needs N %% 64 == 0 (32-row groups of values and gates), N %d", d.N);
+    return DS_OK;
+}
+
 extern "C" size_t ds_gemm_i8_workspace_bytes(const int8_t* A, const int8_t* W, const ds_gemm_i8_desc* desc) {
-    if (!desc) return 0;
+    if (!desc || check_desc(*desc) != DS_OK) return 0;
     const Aligned c = aligned_copies(*desc, A, W);
     return c.bytes_a + c.bytes_w;
 }
@@ -799,12 +810,9 @@ extern "C" int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale
                           void* out, const ds_gemm_i8_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
     DS_CHECK_ARG(desc, "ds_gemm_i8: desc is NULL");
     const ds_gemm_i8_desc d = *desc;
-    DS_CHECK_ARG(d.M >= 0 && d.N >= 0 && d.K >= 0, "ds_gemm_i8: negative size (M %d, N %d, K %d)", d.M, d.N, d.K);
-    DS_CHECK_ARG(d.K <= 131071, "ds_gemm_i8: K %d: the 32-bit sums hold K <= 131071", d.K);
-    DS_CHECK_ARG((d.epilogue & ~(DS_EPI_GEGLU | DS_EPI_SILU | DS_EPI_OUT_F32 | DS_EPI_RES_F32)) == 0, "ds_gemm_i8: epilogue %d", d.epilogue);
+    const int legal = check_desc(d);
+    if (legal != DS_OK) return legal;
     const bool geglu = d.epilogue & DS_EPI_GEGLU;
-    DS_CHECK_ARG(!(geglu && (d.epilogue & DS_EPI_SILU)), "ds_gemm_i8: GEGLU and SiLU exclude each other");
-    DS_CHECK_ARG(!geglu || d.N % 64 == 0, "ds_gemm_i8: GEGLU needs N %% 64 == 0 (32-row groups of values and gates), N %d", d.N);
     DS_CHECK_ARG(!(geglu && residual), "ds_gemm_i8: GEGLU takes no residual");
     if (d.M == 0 || d.N == 0) return DS_OK;
     const int cols = geglu ? d.N / 2 : d.N;

@@ -357,7 +357,7 @@ typedef struct ds_gemm_i8_desc {
  * may be out itself (the same pointer, type and stride).  The products it stands next to: ds_gemm_f16's dense ones (nn.Linear,
  * attention.py:54-57, 379, 399).
  * workspace: NULL, or at least ds_gemm_i8_workspace_bytes(A, W, desc) bytes at a multiple of 16 -- room for copies of operands whose rows are not
- * whole multiples of 16 bytes, where those are worth their time (0 where not).  The results are the same with and without. */
+ * whole multiples of 16 bytes, where those are worth their time (0 where not, and for a desc that ds_gemm_i8 refuses).  The results are the same with and without. */
 size_t ds_gemm_i8_workspace_bytes(const int8_t* A, const int8_t* W, const ds_gemm_i8_desc* desc);
 int ds_gemm_i8(const int8_t* A, const int8_t* W, const float* a_scale, const float* w_scale, const float* bias, const void* residual,
                void* out, const ds_gemm_i8_desc* desc, void* workspace, size_t workspace_bytes, void* stream);

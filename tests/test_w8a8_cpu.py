@@ -140,6 +140,13 @@ def test_product_workspace():
     assert lib.ds_gemm_i8_workspace_bytes(P, P, None) == 0
 
 
+@pytest.mark.parametrize("fields", [dict(K=131072, lda=131073, ldw=131073), dict(epilogue=16), dict(epilogue=DS_EPI_GEGLU, N=997), dict(epilogue=DS_EPI_GEGLU | DS_EPI_SILU, N=1024),
+                                    dict(M=-5), dict(N=-5), dict(K=-5)])
+def test_product_that_is_refused_needs_no_workspace(fields):
+    d = _lib.GemmI8Desc(**dict(dict(M=2057, N=997, K=1273, lda=1273, ldw=1273, ldc=997), **fields))
+    assert _lib.load().ds_gemm_i8_workspace_bytes(P, P, C.byref(d)) == 0
+
+
 NORM = dict(x=P, xt=0, ldx=32, r=P, rt=0, ldr=32, g=P, s=P, lds=32, y=P, yt=2, ldy=32, scale=P, rows=4, C=32, eps=1e-6)
 
 
