@@ -6,6 +6,7 @@ Objects are rebuilt only when a source (or a header) is newer.  The .so stays ne
 travels to the GPU box with the repo snapshot (git-ignored, not gpurun-ignored).
 """
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -100,26 +101,43 @@ def build(force=False, verbose=True, variant=None):
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
     if variant is None:
-        build_torch(verbose)
+        build_torch(force, verbose)
     return lib
 
 
-def build_torch(verbose=True):
-    """_w8a8.so (csrc/w8a8_torch.cpp): the tensor front end of the W8A8 operators, a CPython extension against the installed torch."""
+def build_torch(force=False, verbose=True):
+    """_w8a8.so (csrc/w8a8_torch.cpp): the tensor front end of the W8A8 operators, a CPython extension against the installed torch, built anew where
+    that or the interpreter has changed.  None, and a line on stderr, where there is no torch, none of its headers or no g++: C callers of the library need
+    none of them, and the operators' Python functions say what is missing."""
     import sysconfig
-    import torch
-    from torch.utils.cpp_extension import include_paths
     src = os.path.join(CSRC, "w8a8_torch.cpp")
-    lib = os.path.join(HERE, "_w8a8.so")
-    if _newer([src, os.path.join(HERE, "..", "include", "dynscaler_hip.h")], lib):
+    lib, stamp = os.path.join(HERE, "_w8a8.so"), os.path.join(OBJ, "w8a8.stamp")
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError as e:
+        sys.stderr.write(f"[build] {lib} not built: {e}\n")
+        return None
+    headers = include_paths() + [sysconfig.get_paths()["include"]]
+    for need, found in (("g++", shutil.which("g++")), ("torch's C++ headers", any(os.path.exists(os.path.join(d, "torch", "csrc", "Dtype.h")) for d in headers)),
+                        ("Python.h", os.path.exists(os.path.join(headers[-1], "Python.h")))):
+        if not found:
+            sys.stderr.write(f"[build] {lib} not built: no {need}\n")
+            return None
+    against = f"{torch.__version__} {torch.__file__} {sysconfig.get_config_var('SOABI')}\n"
+    built = open(stamp).read() if os.path.exists(stamp) else None
+    if force or built != against or _newer([src, os.path.join(HERE, "..", "include", "dynscaler_hip.h")], lib):
         cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DUSE_ROCM=1", "-D__HIP_PLATFORM_AMD__=1"]
-               + ["-I" + d for d in include_paths() + [sysconfig.get_paths()["include"], "/opt/rocm/include"]] + [src, "-o", lib]
+               + ["-I" + d for d in headers + ["/opt/rocm/include"]] + [src, "-o", lib]
                + ["-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"])
         r = subprocess.run(cmd, capture_output=True, text=True)
         if verbose and (r.stdout or r.stderr):
             sys.stderr.write(r.stdout + r.stderr)
         if r.returncode != 0:
             raise RuntimeError("g++ failed: " + " ".join(cmd))
+        os.makedirs(OBJ, exist_ok=True)
+        with open(stamp, "w") as f:
+            f.write(against)
     return lib
 
 

@@ -194,3 +194,46 @@ def test_sources_compile_without_warnings(source):
     r = subprocess.run([build.HIPCC] + build.FLAGS + build.SOURCE_FLAGS[source] + ["-Werror", "-Wno-unused-command-line-argument", "--cuda-device-only", "-fsyntax-only",
                                                                                    "-x", "hip", os.path.join(build.CSRC, source)], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+class Compiler:
+    """Stands for subprocess.run in the build: counts the calls, compiles nothing."""
+    def __init__(self):
+        self.calls = 0
+
+    def __call__(self, cmd, **kw):
+        self.calls += 1
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+
+def test_the_front_end_is_built_anew_where_that_is_asked_for_or_torch_has_changed(monkeypatch, tmp_path):
+    from dynamicscaler_amd import build
+    run = Compiler()
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "OBJ", str(tmp_path))
+    monkeypatch.setattr(build, "_newer", lambda sources, target: False)
+    counts = []
+    for force, version in ((False, None), (False, None), (True, None), (False, "99.0"), (False, "99.0")):
+        if version:
+            monkeypatch.setattr(torch, "__version__", version)
+        assert build.build_torch(force=force, verbose=False)
+        counts.append(run.calls)
+    assert counts == [1, 1, 2, 3, 3]
+
+
+@pytest.mark.parametrize("missing", ["torch", "g++", "headers"])
+def test_a_build_without_torch_leaves_out_the_front_end_alone(monkeypatch, missing, capsys):
+    import sys
+    import torch.utils.cpp_extension as ext
+    from dynamicscaler_amd import build
+    run = Compiler()
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "_newer", lambda sources, target: False)
+    if missing == "torch":
+        monkeypatch.setitem(sys.modules, "torch", None)
+    elif missing == "g++":
+        monkeypatch.setattr(build.shutil, "which", lambda name: None)
+    else:
+        monkeypatch.setattr(ext, "include_paths", lambda: [])
+    assert build.build(verbose=False) == build.LIB and run.calls == 0
+    assert "_w8a8.so not built" in capsys.readouterr().err
