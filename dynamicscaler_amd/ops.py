@@ -566,7 +566,7 @@ def gemm_i8(A, W, a_scale, w_scale, bias=None, residual=None, *, out=None, out_d
     DS_EPI_SILU or DS_EPI_GEGLU (N % 64 == 0, W's rows and the bias in 32-row groups of values and gates as for `gemm`; N / 2 output
     columns; no residual).  Any sizes, row strides and alignments; `residual` may be `out` itself."""
     front = _W8A8 or _w8a8()
-    if _timing_hook is None:
+    if _timing_hook is None or not (getattr(A, "ndim", 0) == getattr(W, "ndim", 0) == 2):          # (what is no matrix is refused there)
         return front.gemm_i8(A, W, a_scale, w_scale, bias, residual, out, out_dtype, epilogue, stream)
     made = []
     (M, K), N = A.shape, W.shape[0]

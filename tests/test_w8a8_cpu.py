@@ -49,6 +49,18 @@ def test_product_refuses(change, says):
         ops.gemm_i8(**product(**change))
 
 
+@pytest.mark.parametrize("change,says", [(dict(A=[[1]]), "not a tensor"), (dict(W=None), "not a tensor"), (dict(A=torch.zeros((4, 32, 1), dtype=I8)), "\\[rows, columns\\]"),
+                                         (dict(W=torch.zeros(32, dtype=I8)), "\\[rows, columns\\]"), (dict(A=torch.zeros((), dtype=I8)), "\\[rows, columns\\]"),
+                                         (dict(W=torch.zeros((64, 31), dtype=I8)), "expected 64 x 32"), (dict(), "no CPU fallback")])
+def test_product_refuses_the_same_under_a_timing_hook(change, says):
+    ops.set_timing_hook(lambda name, flops, launch, info: launch())
+    try:
+        with pytest.raises(DsError, match=says):
+            ops.gemm_i8(**product(**change))
+    finally:
+        ops.set_timing_hook(None)
+
+
 X = torch.zeros((4, 32), dtype=F16)
 
 
