@@ -581,6 +581,25 @@ def test_many_rows(m, n):
     close(ops.dequantize_rows_i8(q, scale), v, H32 * v.abs(), F16)
 
 
+@pytest.mark.parametrize("m,n", [(5000, 320), (2051, 1283), (1100, 5120), (300, 16384)])
+def test_many_rows_in_fp32(m, n):
+    """fp32 rows, with and without an fp16 residual, more of them than a launch has teams."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    x, g, r = row_inputs(m, n, 5, F32), 1.0 + 0.2 * normal((n,), n), normal((m, n), 6, F16)
+    one = torch.ones(m, 1, dtype=torch.float64)
+    q, scale = ops.quantize_rows_i8(x.to(d))
+    check_rows_i8(q, scale, x.double(), one)
+    for res in (None, r):
+        h, t, root = rows_ref(x, res, g, 1e-6, True)
+        q, scale, back = ops.rmsnorm_i8(x.to(d), g.to(d), residual=None if res is None else res.to(d))
+        check_rows_i8(q, scale, t, root)
+        y, again = ops.rmsnorm(x.to(d), g.to(d), residual=None if res is None else res.to(d), out_dtype=F32)
+        close(y, t * root, 5 * H32 * (t * root).abs(), F32)
+        if res is not None:
+            assert torch.equal(back.cpu(), once(h)) and torch.equal(again, back)
+
+
 def test_more_rows_than_a_launch_has_threads_for():
     """70 million rows of three values: more workgroups than a grid takes, so each walks several."""
     from dynamicscaler_amd import ops
@@ -793,7 +812,7 @@ def test_product_c_entry_without_a_workspace(m, n, k, flags):
 
 @contextlib.contextmanager
 def at_most(mib):
-    """The allocator may take `mib` MiB more than what is held now."""
+    """The allocator may take `mib` MiB more than what is held now (by a test that began with empty_cache(): its blocks have no free neighbours)."""
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
     torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (mib << 20)) / torch.cuda.get_device_properties(0).total_memory)
@@ -807,6 +826,7 @@ def test_outputs_that_do_not_fit_raise_as_everywhere():
     """torch.OutOfMemoryError, as the other operators' allocations do; the same call goes through once there is room."""
     from dynamicscaler_amd import ops
     d = dev()
+    torch.cuda.empty_cache()
     x, g = torch.ones((50000, 2048), dtype=F16, device=d), torch.ones(2048, device=d)
     q, s = ops.quantize_rows_i8(x)
     calls = [lambda: ops.gemm_i8(q, q[:2048], s, s[:2048]), lambda: ops.rmsnorm(x, g), lambda: ops.rmsnorm_i8(x, g), lambda: ops.quantize_rows_i8(x),
@@ -824,6 +844,7 @@ def test_product_without_room_for_its_workspace():
     """The workspace only makes odd rows quicker: where it cannot be had the call reads them as they lie, with the same bits."""
     from dynamicscaler_amd import ops
     d = dev()
+    torch.cuda.empty_cache()
     a, w, sa, sw, b, _ = [None if t is None else t.to(d) for t in product_case(20057, 1997, 1273, 5)]
     ref = ops.gemm_i8(a, w, sa, sw, bias=b)
     out = torch.zeros_like(ref)
