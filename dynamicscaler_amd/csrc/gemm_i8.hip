@@ -7,9 +7,9 @@
 // Fragments (v_mfma_i32_16x16x64_i8): lane l holds 16 bytes of row l % 16 at k = 16 * (l / 16); the WEIGHT fragment is the first operand,
 // so a lane's accumulator quad is one output row (l % 16) and 4 consecutive columns (4 * (l / 16)).
 //
-// Two kernels: a few rows (bound by how fast a CU can fetch: ~34 GB/s each) and tiles (bound by the matrix cores under the chip's power limit --
-// 8192^3 453 us, 2.43 POP/s; 40960 x 10240 x 1280 with GEGLU 541 us, 1.98 POP/s -- or, for short K, by memory: 655360 x 320 x 320 onto an
-// fp32 residual 380 us, 4.97 TB/s).
+// Two kernels: a few rows (bound by what a CU fetches) and tiles (bound by the matrix cores and, by a third at K = 1280, by what stands before and behind
+// the K loop -- 8192^3 437 us, 2.52 POP/s; 40960 x 10240 x 1280 with GEGLU 568 us, 1.89 POP/s -- or, for short K, by memory: 655360 x 320 x 320
+// onto an fp32 residual 401 us, 4.70 TB/s).
 #include "common.h"
 
 namespace {
@@ -113,9 +113,9 @@ __device__ __forceinline__ float gelu_f(float g) {
     return 0.5f * g * (g < 0.0f ? e : 2.0f - e);
 }
 
-// The same for fp16 results: 1 + erf(g / sqrt 2) is E(|g|) for g < 0 and 2 - E(|g|) otherwise, E(a) = erfc(a / sqrt 2) = 2^-q(a) with a polynomial
-// q of degree 8 (minimax fit on [0, 9], 8.6e-6 off, so E is within 2e-5 of itself and gelu within 2e-6 absolute -- a fortieth and less of an
-// fp16 rounding); behind 9 E < 2.3e-19 counts as zero.  12 vector instructions where erff takes ~40: the GEGLU epilogue is bound by them.
+// The same for fp16 results: E(a) = 2^-q(a) with a polynomial q of degree 8 (least maximum on [0, 9]; 1.2e-5 off with its coefficients in 32 bits, E 1.3e-5 of
+// itself evaluated in them, 2e-5 with the hardware's 2^x, and gelu 2e-6 absolute: a twenty-fifth and less of an fp16 rounding); behind 9 E < 2.3e-19
+// counts as zero.  12 vector instructions where erff takes ~40: the GEGLU epilogue is bound by them.
 __device__ __forceinline__ float gelu_f16(float g) {
     const float a = fabsf(g);
     float q = -7.463252416073374e-08f;
@@ -725,8 +725,8 @@ void launch_few(const I8Args& p, bool odd, hipStream_t st) {
     else gemm_i8_few_kernel<MT, GEGLU, false><<<grid, waves * 64, lds, st>>>(p);
 }
 
-// At most 64 rows: every workgroup of 16 columns reads all of A, so the few-rows kernel's time goes with (16 + M) N K at ~8.5 TB/s (a workgroup alone:
-// 34 GB/s; odd addresses and GEGLU's two weight rows 40 % of that); the 64 x 64 tiles take about as long for one row as for 64, by K,
+// At most 64 rows: every workgroup of 16 columns reads all of A, so the few-rows kernel's time goes with (16 + M) N K at ~8.5 TB/s (a workgroup alone, by
+// the same fit: 34 GB/s; odd addresses and GEGLU's two weight rows 40 % of that); the 64 x 64 tiles take about as long for one row as for 64, by K,
 // while there are no more of them than CUs.  Microseconds of both, within 20 % at 1 ... 64 rows, N = 320 ... 40960, K = 320 ... 4096:
 // 16 x 1280 x 1280 3.3 against 6.0, 64 x 4096 x 4096 12.0 / 12.7, 32 x 10240 x 1280 8.6 / 7.1 (GEGLU 10.3 / 6.4), 48 x 40960 x 1280 26.9 / 12.5,
 // 32 x 4097 x 4095 18.2 / 21, 64 x 4097 x 4095 29.9 / 21.

@@ -7,7 +7,7 @@
 // t is formed and compared in 64 bits and the sums are 64-bit, so q is the correctly rounded quotient (halves to even) of the inputs as
 // they are given: it does not depend on the order of a reduction.  A row without a largest value (all zeros) has q = 0, scale = 0; a row that
 // holds a NaN or an infinity (in x, r or t) has q = 0, scale = NaN: it stands for NaN throughout.
-// fp16 results are rounded once, from the 64-bit value (by way of a rounding to odd: fp16 rows of 655360 x 320 164 us, 159 with two roundings).
+// fp16 results are rounded once, from the 64-bit value (by way of a rounding to odd: fp16 rows of 655360 x 320 164 us a call, 159 with two roundings).
 #include "common.h"
 
 namespace {
@@ -124,9 +124,9 @@ template <> struct Chunk<int8_t> {
 // reduced twice, written once; lane i of the team holds chunks i, i + T, ... of 8 values, so a load covers 16 T contiguous bytes (fp16).
 // A row's last chunk always ends at the row's end: where C % 8 != 0 it overlaps the one before, counts its own values only in the sum, and
 // stores the same bits over the shared ones (every load of a row comes before its first store, also where sum / y lie over an input).
-// A team walks rows `grid` apart and keeps its part of gamma.  Bound by memory: 655360 x 320 with an fp32 residual (11 bytes a value) 461 us = 5.0 TB/s,
-// the quantisation of 40960 x 5120 (3 bytes) 120 us = 5.2 TB/s, where a copy of 4 GiB reaches 4.75.  A few rows are bound by instruction
-// fetch: one row of 1280 takes 3.7 us, of which the launch alone is 1.8, and took 4.9 with an exact branch at every value.
+// A team walks rows `grid` apart and keeps its part of gamma.  Bound by memory: 655360 x 320 with an fp32 residual (11 bytes a value) 474 us = 4.9 TB/s,
+// the quantisation of 40960 x 5120 (3 bytes) 135 us = 4.7 TB/s, where a copy of 4 GiB reaches 4.75.  A few rows are bound by instruction
+// fetch: one row of 1280 takes 3.5 us, of which the launch alone is 1.8, and took 4.9 with an exact branch at every value.
 template <typename X, typename R, typename Y, bool NORM, bool RES, int T, int V>
 __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p, int rows) {
     constexpr int TEAMS = T > 256 ? 1 : 256 / T, WAVES = T / 64;
@@ -329,8 +329,9 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p, int rows) {
 }
 
 // The chunks of 8 values of all rows in one sequence, `span` of them a workgroup (per_row of them a row; magic: i / per_row = i * magic >> 40 for
-// i < per_row + span, both < 2^16): every lane has work whatever the row's length.  C >= 8; a row's last chunk ends at the row's end.  655360 x 320 to fp16 110 us (5.7 TB/s; with
-// a second rounding in place of the odd one 108), with teams of 64 lanes a row, 40 of them at work, 186 us before that.
+// i < per_row + span, both < 2^16): every lane has work whatever the row's length.  C >= 8; a row's last chunk ends at the row's end.  655360 x 320 to fp16
+// 106 us (5.9 TB/s; 3001 x 1283, in the cache, 4.2 us, 3.7 with two roundings in place of the odd one); teams of 64 lanes a row, 40 of them at work,
+// took 186.
 template <typename Y>
 __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__ q8, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C,
                                                       unsigned per_row, unsigned long long magic, int span) {

@@ -342,7 +342,8 @@ int ds_silu_f16(const void* x, void* y, size_t n, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * W8A8: 8-bit integer operands with one fp32 scale per row -- of the activations a token's, of the weights an output channel's.  A
- * transformer block's chain: ds_rmsnorm_rows (8-bit) -> ds_gemm_i8 (GEGLU) -> ds_quantize_rows_i8 -> ds_gemm_i8 (+ residual).
+ * feed-forward's chain: ds_rmsnorm_rows (8-bit; behind a LayerNorm ds_quantize_rows_i8) -> ds_gemm_i8 (GEGLU) -> ds_quantize_rows_i8 ->
+ * ds_gemm_i8 (+ residual).
  * Row strides (ld*) are in elements, >= the row's length, otherwise free; pointers have to be aligned to their element only.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct ds_gemm_i8_desc {
