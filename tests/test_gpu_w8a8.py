@@ -665,6 +665,27 @@ def test_feed_forward_of_a_block(rows, width, rt):
     assert float((branch - f).norm() / f.norm()) <= 0.04
 
 
+@pytest.mark.parametrize("rows,width", [(1, 64), (77, 320), (300, 1280)])
+def test_feed_forward_behind_a_layernorm(rows, width):
+    """The chain of a block with a LayerNorm: its fp16 rows are quantised, every link against its definition on the inputs it was given."""
+    from dynamicscaler_amd import ops
+    d = dev()
+    p, _, _ = block(width, 70, d)
+    stream = normal((rows, width), 1, F32, 2.0).to(d)
+    x = ops.layernorm(stream, p["g"], torch.zeros(width, device=d))
+    q, s = ops.quantize_rows_i8(x)
+    hidden = ops.gemm_i8(q, p["w1"], s, p["s1"], bias=p["b1"], epilogue=EPI["geglu"])
+    q2, s2 = ops.quantize_rows_i8(hidden)
+    before = stream.cpu().clone()
+    ops.gemm_i8(q2, p["w2"], s2, p["s2"], bias=p["b2"], residual=stream, out=stream)
+    one = torch.ones(rows, 1, dtype=torch.float64)
+    check_rows_i8(q, s, x.cpu().double(), one)
+    c = {k: v.cpu() for k, v in p.items()}
+    close(hidden, *product_ref(q.cpu(), c["w1"], s.cpu(), c["s1"], c["b1"], None, "geglu"), F16)
+    check_rows_i8(q2, s2, hidden.cpu().double(), one)
+    close(stream, *product_ref(q2.cpu(), c["w2"], s2.cpu(), c["s2"], c["b2"], before, "none"), F32)
+
+
 def test_feed_forward_in_a_graph_and_on_two_streams():
     """A captured block replayed between eager work, and two blocks at once on two streams: every result equals the eager one."""
     d = dev()
@@ -812,12 +833,13 @@ def test_product_c_entry_without_a_workspace(m, n, k, flags):
 
 @contextlib.contextmanager
 def at_most(mib):
-    """The allocator may take `mib` MiB more than what is held now (by a test that began with empty_cache(): its blocks have no free neighbours)."""
+    """The allocator may take `mib` MiB more than what is held now, and gives nothing out of that (a pool of its own)."""
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
     torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (mib << 20)) / torch.cuda.get_device_properties(0).total_memory)
     try:
-        yield
+        with torch.cuda.use_mem_pool(torch.cuda.MemPool()):
+            yield
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
 
@@ -826,7 +848,6 @@ def test_outputs_that_do_not_fit_raise_as_everywhere():
     """torch.OutOfMemoryError, as the other operators' allocations do; the same call goes through once there is room."""
     from dynamicscaler_amd import ops
     d = dev()
-    torch.cuda.empty_cache()
     x, g = torch.ones((50000, 2048), dtype=F16, device=d), torch.ones(2048, device=d)
     q, s = ops.quantize_rows_i8(x)
     calls = [lambda: ops.gemm_i8(q, q[:2048], s, s[:2048]), lambda: ops.rmsnorm(x, g), lambda: ops.rmsnorm_i8(x, g), lambda: ops.quantize_rows_i8(x),
@@ -844,7 +865,6 @@ def test_product_without_room_for_its_workspace():
     """The workspace only makes odd rows quicker: where it cannot be had the call reads them as they lie, with the same bits."""
     from dynamicscaler_amd import ops
     d = dev()
-    torch.cuda.empty_cache()
     a, w, sa, sw, b, _ = [None if t is None else t.to(d) for t in product_case(20057, 1997, 1273, 5)]
     ref = ops.gemm_i8(a, w, sa, sw, bias=b)
     out = torch.zeros_like(ref)
