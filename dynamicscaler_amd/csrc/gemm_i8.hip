@@ -8,8 +8,8 @@
 // so a lane's accumulator quad is one output row (l % 16) and 4 consecutive columns (4 * (l / 16)).
 //
 // Two kernels: a few rows (bound by what a CU fetches) and tiles (bound by the matrix cores and, by a third at K = 1280, by what stands before and behind
-// the K loop -- 8192^3 437 us, 2.52 POP/s; 40960 x 10240 x 1280 with GEGLU 568 us, 1.89 POP/s -- or, for short K, by memory: 655360 x 320 x 320
-// onto an fp32 residual 401 us, 4.70 TB/s).
+// the K loop -- 8192^3 433 us, 2.54 POP/s; 40960 x 10240 x 1280 with GEGLU 550 us, 1.95 POP/s -- or, for short K, by memory: 655360 x 320 x 320
+// onto an fp32 residual 396 us, 4.77 TB/s).
 #include "common.h"
 
 namespace {

@@ -124,8 +124,8 @@ template <> struct Chunk<int8_t> {
 // reduced twice, written once; lane i of the team holds chunks i, i + T, ... of 8 values, so a load covers 16 T contiguous bytes (fp16).
 // A row's last chunk always ends at the row's end: where C % 8 != 0 it overlaps the one before, counts its own values only in the sum, and
 // stores the same bits over the shared ones (every load of a row comes before its first store, also where sum / y lie over an input).
-// A team walks rows `grid` apart and keeps its part of gamma.  Bound by memory: 655360 x 320 with an fp32 residual (11 bytes a value) 474 us = 4.9 TB/s,
-// the quantisation of 40960 x 5120 (3 bytes) 135 us = 4.7 TB/s, where a copy of 4 GiB reaches 4.75.  A few rows are bound by instruction
+// A team walks rows `grid` apart and keeps its part of gamma.  Bound by memory: 655360 x 320 with an fp32 residual (11 bytes a value) 472 us = 4.9 TB/s,
+// the quantisation of 40960 x 5120 (3 bytes) 134 us = 4.7 TB/s, where a copy of 4 GiB reaches 4.75.  A few rows are bound by instruction
 // fetch: one row of 1280 takes 3.5 us, of which the launch alone is 1.8, and took 4.9 with an exact branch at every value.
 template <typename X, typename R, typename Y, bool NORM, bool RES, int T, int V>
 __global__ void __launch_bounds__(T > 256 ? T : 256) rows_team_kernel(RowsArgs p, int rows) {
@@ -329,30 +329,52 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowsArgs p, int rows) {
 }
 
 // The chunks of 8 values of all rows in one sequence, `span` of them a workgroup (per_row of them a row; magic: i / per_row = i * magic >> 40 for
-// i < per_row + span, both < 2^16): every lane has work whatever the row's length.  C >= 8; a row's last chunk ends at the row's end.  655360 x 320 to fp16
-// 106 us (5.9 TB/s; 3001 x 1283, in the cache, 4.2 us, 3.7 with two roundings in place of the odd one); teams of 64 lanes a row, 40 of them at work,
-// took 186.
+// i < per_row + span, both < 2^16): every lane has work whatever the row's length, and its loads are all on their way before the first product.  C >= 8;
+// a row's last chunk ends at the row's end.  655360 x 320 to fp16 105 us a call (6.0 TB/s; 113 with each product rounded to odd), to fp32 208 (270 with
+// the loads a turn apart); 3001 x 1283, in the cache, 3.8 us (4.2).
 template <typename Y>
 __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* __restrict__ q8, long ldq, const float* __restrict__ scale, Y* __restrict__ y, long ldy, int rows, int C,
                                                       unsigned per_row, unsigned long long magic, int span) {
     const unsigned long long first = (unsigned long long)blockIdx.x * span;
     const long row0 = first / per_row;
     const unsigned in0 = (unsigned)(first - row0 * per_row);
-#pragma unroll 4
-    for (int k = threadIdx.x; k < span; k += 256) {
-        const unsigned i = in0 + k, r = (unsigned)((i * magic) >> 40);
-        const long row = row0 + r;
-        if (row >= rows) break;
-        const int c = min((int)(i - r * per_row) * 8, C - 8);
-        const float s = scale[row];
-        const u32x2 v = *reinterpret_cast<const u32x2_u*>(q8 + row * ldq + c);
+    constexpr int TURNS = 4;
+    long row[TURNS];
+    int c[TURNS];
+    float s[TURNS];
+    u32x2 v[TURNS];
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+        if (256 * t >= span) break;
+        const unsigned i = in0 + threadIdx.x + 256 * t, r = (unsigned)((i * magic) >> 40);
+        row[t] = row0 + r;
+        c[t] = min((int)(i - r * per_row) * 8, C - 8);
+        if (row[t] < rows) {
+            s[t] = scale[row[t]];
+            v[t] = *reinterpret_cast<const u32x2_u*>(q8 + row[t] * ldq + c[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+        if (256 * t >= span || row[t] >= rows) break;
+        auto q = [&](int j) { return (float)((int)(v[t][j >> 2] << (24 - 8 * (j & 3))) >> 24); };
         Chunk<Y> cy;
+        // fp16: a product whose fp32 rounding lies halfway between two results (one in 8192; anything of a row with subnormal ones) is rounded to odd
+        bool again = sizeof(Y) == 2 && !(fabsf(s[t]) >= 0x1p-14f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float q = (float)((int)(v[j >> 2] << (24 - 8 * (j & 3))) >> 24), p = q * s;
-            cy.set(j, sizeof(Y) == 2 ? to_odd(p, fmaf(q, s, -p)) : p);
+            const float p = q(j) * s[t];
+            cy.set(j, p);
+            again |= sizeof(Y) == 2 && (__float_as_uint(p) & 0x1fff) == 0x1000;
         }
-        cy.store(y + row * ldy + c);
+        if (sizeof(Y) == 2 && again) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = q(j) * s[t];
+                cy.set(j, to_odd(p, fmaf(q(j), s[t], -p)));
+            }
+        }
+        cy.store(y + row[t] * ldy + c[t]);
     }
 }
 
